@@ -211,6 +211,85 @@ VA_API int va_paged_prefill(void *out, const void *q, const void *k_cache, const
                      void *stream);
 
 /* ---------------------------------------------------------------------------
+ * 8-bit KV cache and windowed attention
+ *
+ * An e4m3 cache holds one byte per value in the layouts of the fp16 cache
+ * (strides s_* in elements, multiples of 16) and one exponent byte per (token,
+ * kv head) in k_scale / v_scale at (block, head, offset) through the strides
+ * sc_block, sc_head, sc_token.  A row of head_size codes c with exponent byte b
+ * stands for c * 2^(b - 127).  The writers below choose, for a row whose largest
+ * finite magnitude is a, the smallest exponent in [-14, 7] with
+ * a <= 448 * 2^(b - 127), round each value once to the nearest e4m3 and saturate
+ * what is larger (infinities, values past 57344); NaN stays NaN.  Every stored
+ * value is an fp16 value, so reading back is exact.  Bytes outside [113, 134]
+ * are not written by this library and are not meaningful to it.
+ *
+ * A query at position p sees the keys j <= p with p - j < window (window <= 0:
+ * every j <= p) or j < sink_tokens.  Blocks that hold no visible key are not
+ * read; their block-table entries may hold anything.  Keys that are not visible
+ * do not reach the result, whatever their values.
+ * ------------------------------------------------------------------------- */
+
+/* Quantise new K/V rows [num_tokens, num_kv_heads, head_size] (fp16, element
+ * strides new_s_*) and scatter them by slot = block*block_size + offset.
+ * slot == -1 is padding and skipped; any other slot outside the cache is skipped
+ * and flagged.  Live slots must be distinct: of a slot named twice the row is
+ * undefined.  head_size 32, 64, 96 or 128; any block_size. */
+VA_API int va_kv_quant_write_slots(void *k_cache, void *v_cache, void *k_scale, void *v_scale,
+                                   const void *new_k, const void *new_v,
+                                   const void *slot_mapping, int slot_is_i64,
+                                   int64_t num_tokens, int num_kv_heads, int head_size,
+                                   int block_size, int64_t num_blocks, int64_t s_block,
+                                   int64_t s_head, int64_t s_token, int64_t sc_block,
+                                   int64_t sc_head, int64_t sc_token, int64_t new_s_token,
+                                   int64_t new_s_head, int32_t *err_flag, void *stream);
+
+/* Read the active rows of an e4m3 cache back into an fp16 cache: position t <
+ * seq_lens[s] of sequence s goes from block block_table[s][t/bs] of the source to
+ * block dst_block_table[s][t/bs] (NULL: the same id) of the destination, exactly.
+ * Rows past a sequence's end are left as they are.  A block id outside its cache
+ * is skipped and flagged; a sequence longer than the table is skipped and flagged. */
+VA_API int va_kv_dequant_blocks(const void *src_k, const void *src_v, const void *k_scale,
+                                const void *v_scale, void *dst_k, void *dst_v,
+                                const int32_t *block_table, const int32_t *dst_block_table,
+                                const int32_t *seq_lens, int64_t num_seqs,
+                                int64_t max_blocks_per_seq, int num_kv_heads, int head_size,
+                                int block_size, int64_t src_num_blocks, int64_t dst_num_blocks,
+                                int64_t src_s_block, int64_t src_s_head, int64_t src_s_token,
+                                int64_t sc_block, int64_t sc_head, int64_t sc_token,
+                                int64_t dst_s_block, int64_t dst_s_head, int64_t dst_s_token,
+                                int32_t *err_flag, void *stream);
+
+/* Bytes of workspace va_window_decode needs for this shape (fp32 partials of
+ * sequences cut over several CTAs; 0 when none is cut).  No initialisation
+ * needed; calls that share a workspace must not overlap on the GPU. */
+VA_API size_t va_window_decode_workspace_size(int64_t num_seqs, int num_query_heads,
+                                              int num_kv_heads, int head_size,
+                                              int64_t max_seq_len, int window, int sink_tokens);
+
+/* Single-token attention over the visible keys of each sequence, with the write
+ * of the new row.  The arguments are va_paged_decode's, with kv_e4m3 (0: fp16
+ * cache, k_scale / v_scale ignored; 1: e4m3 cache), any block_size >= 1, window
+ * and sink_tokens; scale must be positive and finite.  When new_k / new_v are
+ * given, row i is written to position seq_lens[i]-1 (quantised for an e4m3 cache)
+ * and the attention reads what was written.  Rows with seq_len <= 0 are skipped;
+ * rows whose length exceeds max_seq_len or the block table, or whose visible keys
+ * lie in a block outside the cache, are flagged and their output is left as it
+ * is.  q, new_k, new_v and cache rows start on 16-byte boundaries. */
+VA_API int va_window_decode(void *out, const void *q, void *k_cache, void *v_cache,
+                            void *k_scale, void *v_scale, int kv_e4m3,
+                            const int32_t *block_table, const int32_t *seq_lens,
+                            const void *new_k, const void *new_v, int64_t num_seqs,
+                            int num_query_heads, int num_kv_heads, int head_size,
+                            int block_size, int64_t max_blocks_per_seq, int64_t max_seq_len,
+                            int64_t num_blocks, float scale, int window, int sink_tokens,
+                            int64_t s_block, int64_t s_head, int64_t s_token, int64_t sc_block,
+                            int64_t sc_head, int64_t sc_token, int64_t q_s_token,
+                            int64_t q_s_head, int64_t o_s_token, int64_t o_s_head,
+                            int64_t new_s_token, int64_t new_s_head, void *workspace,
+                            size_t workspace_bytes, int32_t *err_flag, void *stream);
+
+/* ---------------------------------------------------------------------------
  * Step-level ops around the attention call
  * ------------------------------------------------------------------------- */
 

@@ -1,0 +1,64 @@
+// e4m3 rows with one power-of-two scale: device helpers of the 8-bit KV cache.
+//
+// A row is the head_size values of one token and one kv head.  With a = the largest
+// finite |x| of the row, its exponent is e = ceil(log2(a / 448)) clamped to [-14, 7]
+// (-14 for a row of zeros): the smallest e in that range with a <= 448 * 2^e.  The row
+// is stored as the e4m3 codes of x * 2^-e and one byte e + 127.
+//
+// Why a power of two: x * 2^-e is exact in fp32, so the code is x rounded ONCE, to the
+// nearest e4m3 (half a step, 2^-4 relative).  Why that range: a code is a multiple of
+// 2^-9 up to 448, so code * 2^e is a multiple of 2^-23 up to 57344, an fp16 value for
+// every e -- reading back is exact, and the attention kernels feed the tensor cores
+// code * 2^e in fp16 without a second rounding.  Values past 57344 (and infinities)
+// saturate; NaN stays NaN.
+#pragma once
+
+#include "common.cuh"
+
+namespace va {
+
+constexpr int kQ8ExpBias = 127;
+
+// Largest finite |x| of a packed fp16 pair, as fp16 bits per half, folded into `m`
+// (magnitudes of one sign order like their bits).
+VA_DEVINL uint32_t q8_absmax2(uint32_t m, uint32_t w) {
+  uint32_t a = w & 0x7fff7fffu;
+  a &= __vcmpltu2(a, 0x7c007c00u);
+  return __vmaxu2(m, a);
+}
+
+// Exponent of a row whose largest finite magnitude has the fp16 bits `amax`.
+VA_DEVINL int q8_exponent(uint32_t amax) {
+  const uint32_t b = __float_as_uint(__half2float(__ushort_as_half((unsigned short)amax)));
+  // a = f * 2^E, 1 <= f < 2; 448 = 1.75 * 2^8
+  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return min(max(e, -14), 7);
+}
+
+VA_DEVINL float q8_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// fp16 bits of 2^e, from the stored byte e + 127 (e in [-14, 7]), in both halves.
+VA_DEVINL uint32_t q8_scale_h2(uint32_t byte) { return ((byte - 112u) << 10 & 0xffffu) * 0x10001u; }
+
+// Two fp16 values times inv (a power of two), as two e4m3 codes (low half -> low byte).
+VA_DEVINL uint32_t q8_encode2(uint32_t h2, float inv) {
+  const float2 f = h2_to_f2(h2);
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(f.y * inv), "f"(f.x * inv));
+  return r;
+}
+
+// Two e4m3 codes (the low 16 bits of `c`) as fp16, low byte -> low half.
+VA_DEVINL uint32_t q8_decode2(uint32_t c) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)c));
+  return r;
+}
+
+VA_DEVINL uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+}  // namespace va

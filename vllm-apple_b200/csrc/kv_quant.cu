@@ -1,0 +1,306 @@
+// The 8-bit KV cache: rows quantised as they are written, and read back to fp16.
+// (Row format and its reasons: kv_q8.cuh.)
+//
+// Both kernels move each byte once and are bound by HBM (small calls by the launch).
+#include "kv_q8.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// ---------------------------------------------------------------------------
+// write: fp16 rows -> codes + exponent byte, scattered by slot
+// ---------------------------------------------------------------------------
+struct QWriteArgs {
+  uint8_t *kc, *vc, *ks, *vs;
+  const __half *nk, *nv;
+  const void *slots;
+  int slot64, heads, bs;
+  int64_t rows, num_slots;  // rows = tokens * heads
+  int64_t s_block, s_head, s_token, c_block, c_head, c_token, n_token, n_head;
+  int32_t *err;
+};
+
+// A group of L lanes owns one (token, head): every lane takes 8 values (16 bytes) of the
+// K row and of the V row, so a row is read once, its maximum is a shuffle reduction and
+// the codes never leave registers.  head_size 96 leaves 4 of 16 lanes idle.
+template <int D>
+__global__ void __launch_bounds__(kThreads) kv_quant_write_kernel(const QWriteArgs a) {
+  constexpr int L = D > 64 ? 16 : D / 8;
+  va::pdl_enter();
+  const int sub = threadIdx.x % L;
+  const bool on = sub * 8 < D;
+  const int64_t step = (int64_t)gridDim.x * (kThreads / L);
+  for (int64_t row0 = (int64_t)blockIdx.x * (kThreads / L); row0 < a.rows; row0 += step) {
+    const int64_t row = row0 + threadIdx.x / L;
+    const bool in = row < a.rows;
+    int64_t tok = 0;
+    int h = 0;
+    int64_t slot = -1;
+    if (in) {
+      if (a.rows <= INT32_MAX) {
+        tok = (uint32_t)row / (uint32_t)a.heads;
+      } else {
+        tok = row / a.heads;
+      }
+      h = (int)(row - tok * a.heads);
+      slot = a.slot64 ? __ldg(static_cast<const int64_t *>(a.slots) + tok)
+                      : (int64_t)__ldg(static_cast<const int32_t *>(a.slots) + tok);
+      if (slot < -1 || slot >= a.num_slots) {
+        if (h == 0 && sub == 0) va::raise_flag(a.err, VA_FLAG_BAD_SLOT);
+        slot = -1;
+      }
+    }
+    uint4 k = make_uint4(0, 0, 0, 0), v = k;
+    if (slot >= 0 && on) {
+      const int64_t src = tok * a.n_token + (int64_t)h * a.n_head + sub * 8;
+      k = __ldcs(reinterpret_cast<const uint4 *>(a.nk + src));
+      v = __ldcs(reinterpret_cast<const uint4 *>(a.nv + src));
+    }
+    uint32_t mk = 0, mv = 0;
+    mk = va::q8_absmax2(va::q8_absmax2(va::q8_absmax2(va::q8_absmax2(0, k.x), k.y), k.z), k.w);
+    mv = va::q8_absmax2(va::q8_absmax2(va::q8_absmax2(va::q8_absmax2(0, v.x), v.y), v.z), v.w);
+    // one 16-bit maximum each, K in the low half and V in the high half
+    uint32_t m = max(mk & 0xffffu, mk >> 16) | max(mv & 0xffffu, mv >> 16) << 16;
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (slot < 0) continue;
+    const int ek = va::q8_exponent(m & 0xffffu), ev = va::q8_exponent(m >> 16);
+    const float ik = va::q8_pow2(-ek), iv = va::q8_pow2(-ev);
+    int64_t blk, off;
+    if (slot <= INT32_MAX) {
+      blk = (uint32_t)slot / (uint32_t)a.bs;
+    } else {
+      blk = slot / a.bs;
+    }
+    off = slot - blk * a.bs;
+    if (on) {
+      const int64_t dst = blk * a.s_block + h * a.s_head + off * a.s_token + sub * 8;
+      uint2 ck, cv;
+      ck.x = va::q8_encode2(k.x, ik) | va::q8_encode2(k.y, ik) << 16;
+      ck.y = va::q8_encode2(k.z, ik) | va::q8_encode2(k.w, ik) << 16;
+      cv.x = va::q8_encode2(v.x, iv) | va::q8_encode2(v.y, iv) << 16;
+      cv.y = va::q8_encode2(v.z, iv) | va::q8_encode2(v.w, iv) << 16;
+      *reinterpret_cast<uint2 *>(a.kc + dst) = ck;
+      *reinterpret_cast<uint2 *>(a.vc + dst) = cv;
+    }
+    if (sub == 0) {
+      const int64_t c = blk * a.c_block + h * a.c_head + off * a.c_token;
+      a.ks[c] = (uint8_t)(ek + va::kQ8ExpBias);
+      a.vs[c] = (uint8_t)(ev + va::kQ8ExpBias);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// read: active blocks -> fp16 cache
+// ---------------------------------------------------------------------------
+struct QReadArgs {
+  const uint8_t *kc, *vc, *ks, *vs;
+  __half *dk, *dv;
+  const int32_t *bt, *dbt, *sl;
+  int heads, bs, bpu;  // bpu: blocks per unit
+  int head_minor;      // walk tokens outermost (rows of one token lie together)
+  int64_t num_seqs, max_blocks, units_per_seq, src_nb, dst_nb;
+  int64_t s_block, s_head, s_token, c_block, c_head, c_token, d_block, d_head, d_token;
+  int32_t *err;
+};
+
+// A CTA takes `bpu` consecutive blocks of one sequence (a unit) and walks them in pieces
+// of 16 codes in the order the source stores them; a piece of K and the same piece of V
+// are in flight together, four times per thread before the first is used.
+template <int D>
+__global__ void __launch_bounds__(kThreads) kv_dequant_kernel(const QReadArgs a) {
+  constexpr int P = D / 16;  // pieces per row
+  constexpr int U = 4;
+  va::pdl_enter();
+  const int64_t units = a.num_seqs * a.units_per_seq;
+  const int rows_blk = a.heads * a.bs;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int64_t seq = u / a.units_per_seq;
+    const int64_t b0 = (u - seq * a.units_per_seq) * a.bpu;
+    const int64_t n = __ldg(a.sl + seq);
+    if (n <= 0) continue;
+    const int64_t nblk = (n + a.bs - 1) / a.bs;
+    if (nblk > a.max_blocks) {
+      if (b0 == 0 && threadIdx.x == 0) va::raise_flag(a.err, VA_FLAG_CTX_OVERFLOW);
+      continue;
+    }
+    const int nb = (int)min((int64_t)a.bpu, nblk - b0);  // <= 0 past the sequence
+    const int total = nb * rows_blk * P;
+    for (int i0 = threadIdx.x; i0 < total; i0 += kThreads * U) {
+      uint4 k[U], v[U];
+      uint32_t fk[U], fv[U];
+      int64_t dst[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int i = i0 + j * kThreads;
+        dst[j] = -1;
+        if (i >= total) continue;
+        const int r = i / P, c = i - r * P;
+        const int b = (uint32_t)r / (uint32_t)rows_blk, rb = r - b * rows_blk;
+        int h, t;
+        if (a.head_minor) {
+          t = (uint32_t)rb / (uint32_t)a.heads;
+          h = rb - t * a.heads;
+        } else {
+          h = (uint32_t)rb / (uint32_t)a.bs;
+          t = rb - h * a.bs;
+        }
+        if ((b0 + b) * a.bs + t >= n) continue;
+        const int64_t e = seq * a.max_blocks + b0 + b;
+        const int32_t sb = __ldg(a.bt + e), db = a.dbt ? __ldg(a.dbt + e) : sb;
+        if (sb < 0 || sb >= a.src_nb || db < 0 || db >= a.dst_nb) {
+          if (rb == 0 && c == 0) va::raise_flag(a.err, VA_FLAG_BAD_BLOCK);
+          continue;
+        }
+        const int64_t src = sb * a.s_block + h * a.s_head + t * a.s_token + c * 16;
+        const int64_t sc = sb * a.c_block + h * a.c_head + t * a.c_token;
+        k[j] = __ldcs(reinterpret_cast<const uint4 *>(a.kc + src));
+        v[j] = __ldcs(reinterpret_cast<const uint4 *>(a.vc + src));
+        fk[j] = __ldg(a.ks + sc);
+        fv[j] = __ldg(a.vs + sc);
+        dst[j] = db * a.d_block + h * a.d_head + t * a.d_token + c * 16;
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        if (dst[j] < 0) continue;
+        auto put = [](__half *p, const uint4 &w, uint32_t f) {
+          uint4 lo, hi;
+          lo.x = va::hmul2(va::q8_decode2(w.x), f);
+          lo.y = va::hmul2(va::q8_decode2(w.x >> 16), f);
+          lo.z = va::hmul2(va::q8_decode2(w.y), f);
+          lo.w = va::hmul2(va::q8_decode2(w.y >> 16), f);
+          hi.x = va::hmul2(va::q8_decode2(w.z), f);
+          hi.y = va::hmul2(va::q8_decode2(w.z >> 16), f);
+          hi.z = va::hmul2(va::q8_decode2(w.w), f);
+          hi.w = va::hmul2(va::q8_decode2(w.w >> 16), f);
+          __stcs(reinterpret_cast<uint4 *>(p), lo);
+          __stcs(reinterpret_cast<uint4 *>(p) + 1, hi);
+        };
+        put(a.dk + dst[j], k[j], va::q8_scale_h2(fk[j]));
+        put(a.dv + dst[j], v[j], va::q8_scale_h2(fv[j]));
+      }
+    }
+  }
+}
+
+bool head_size_ok(int D) { return D == 32 || D == 64 || D == 96 || D == 128; }
+bool mult(int64_t s, int64_t m) { return s % m == 0; }
+
+}  // namespace
+
+extern "C" int va_kv_quant_write_slots(void *k_cache, void *v_cache, void *k_scale, void *v_scale,
+                                       const void *new_k, const void *new_v,
+                                       const void *slot_mapping, int slot_is_i64,
+                                       int64_t num_tokens, int num_kv_heads, int head_size,
+                                       int block_size, int64_t num_blocks, int64_t s_block,
+                                       int64_t s_head, int64_t s_token, int64_t sc_block,
+                                       int64_t sc_head, int64_t sc_token, int64_t new_s_token,
+                                       int64_t new_s_head, int32_t *err_flag, void *stream) {
+  if (num_tokens < 0 || num_blocks < 0 || num_kv_heads <= 0 || block_size <= 0)
+    return VA_ERR_INVALID_ARG;
+  if (num_tokens == 0) return VA_OK;
+  if (!k_cache || !v_cache || !k_scale || !v_scale || !new_k || !new_v || !slot_mapping)
+    return VA_ERR_INVALID_ARG;
+  if (!head_size_ok(head_size)) return VA_ERR_UNSUPPORTED;
+  if (num_tokens > (INT64_MAX >> 16) / num_kv_heads) return VA_ERR_UNSUPPORTED;
+  if (!va_host::aligned16(k_cache) || !va_host::aligned16(v_cache) ||
+      !va_host::aligned16(new_k) || !va_host::aligned16(new_v) || !mult(s_block, 16) ||
+      !mult(s_head, 16) || !mult(s_token, 16) || !mult(new_s_token, 8) || !mult(new_s_head, 8))
+    return VA_ERR_INVALID_ARG;
+  QWriteArgs a{};
+  a.kc = static_cast<uint8_t *>(k_cache);
+  a.vc = static_cast<uint8_t *>(v_cache);
+  a.ks = static_cast<uint8_t *>(k_scale);
+  a.vs = static_cast<uint8_t *>(v_scale);
+  a.nk = static_cast<const __half *>(new_k);
+  a.nv = static_cast<const __half *>(new_v);
+  a.slots = slot_mapping;
+  a.slot64 = slot_is_i64;
+  a.heads = num_kv_heads;
+  a.bs = block_size;
+  a.rows = num_tokens * num_kv_heads;
+  a.num_slots = num_blocks * block_size;
+  a.s_block = s_block; a.s_head = s_head; a.s_token = s_token;
+  a.c_block = sc_block; a.c_head = sc_head; a.c_token = sc_token;
+  a.n_token = new_s_token; a.n_head = new_s_head;
+  a.err = err_flag;
+  const int per = kThreads / (head_size > 64 ? 16 : head_size / 8);
+  const int64_t want = (a.rows + per - 1) / per;
+  const dim3 grid((unsigned)(want < (1 << 20) ? want : (1 << 20)));
+  auto st = static_cast<cudaStream_t>(stream);
+  int rc = 1;
+  switch (head_size) {
+    case 32: rc = va_host::launch_pdl(kv_quant_write_kernel<32>, grid, kThreads, st, a); break;
+    case 64: rc = va_host::launch_pdl(kv_quant_write_kernel<64>, grid, kThreads, st, a); break;
+    case 96: rc = va_host::launch_pdl(kv_quant_write_kernel<96>, grid, kThreads, st, a); break;
+    case 128: rc = va_host::launch_pdl(kv_quant_write_kernel<128>, grid, kThreads, st, a); break;
+  }
+  return rc ? VA_ERR_LAUNCH : va_host::launch_status();
+}
+
+extern "C" int va_kv_dequant_blocks(const void *src_k, const void *src_v, const void *k_scale,
+                                    const void *v_scale, void *dst_k, void *dst_v,
+                                    const int32_t *block_table, const int32_t *dst_block_table,
+                                    const int32_t *seq_lens, int64_t num_seqs,
+                                    int64_t max_blocks_per_seq, int num_kv_heads, int head_size,
+                                    int block_size, int64_t src_num_blocks,
+                                    int64_t dst_num_blocks, int64_t src_s_block,
+                                    int64_t src_s_head, int64_t src_s_token, int64_t sc_block,
+                                    int64_t sc_head, int64_t sc_token, int64_t dst_s_block,
+                                    int64_t dst_s_head, int64_t dst_s_token, int32_t *err_flag,
+                                    void *stream) {
+  if (num_seqs < 0 || max_blocks_per_seq < 0 || src_num_blocks < 0 || dst_num_blocks < 0 ||
+      num_kv_heads <= 0 || block_size <= 0)
+    return VA_ERR_INVALID_ARG;
+  if (num_seqs == 0 || max_blocks_per_seq == 0) return VA_OK;
+  if (!src_k || !src_v || !k_scale || !v_scale || !dst_k || !dst_v || !block_table || !seq_lens)
+    return VA_ERR_INVALID_ARG;
+  if (!head_size_ok(head_size)) return VA_ERR_UNSUPPORTED;
+  // one block's pieces are counted in 32 bits
+  if ((int64_t)num_kv_heads * block_size > (1 << 24)) return VA_ERR_UNSUPPORTED;
+  if (num_seqs > INT32_MAX || max_blocks_per_seq > INT32_MAX) return VA_ERR_UNSUPPORTED;
+  if (!va_host::aligned16(src_k) || !va_host::aligned16(src_v) || !va_host::aligned16(dst_k) ||
+      !va_host::aligned16(dst_v) || !mult(src_s_block, 16) || !mult(src_s_head, 16) ||
+      !mult(src_s_token, 16) || !mult(dst_s_block, 8) || !mult(dst_s_head, 8) ||
+      !mult(dst_s_token, 8))
+    return VA_ERR_INVALID_ARG;
+  QReadArgs a{};
+  a.kc = static_cast<const uint8_t *>(src_k);
+  a.vc = static_cast<const uint8_t *>(src_v);
+  a.ks = static_cast<const uint8_t *>(k_scale);
+  a.vs = static_cast<const uint8_t *>(v_scale);
+  a.dk = static_cast<__half *>(dst_k);
+  a.dv = static_cast<__half *>(dst_v);
+  a.bt = block_table;
+  a.dbt = dst_block_table;
+  a.sl = seq_lens;
+  a.heads = num_kv_heads;
+  a.bs = block_size;
+  a.head_minor = src_s_head < src_s_token ? 1 : 0;
+  a.num_seqs = num_seqs;
+  a.max_blocks = max_blocks_per_seq;
+  a.src_nb = src_num_blocks;
+  a.dst_nb = dst_num_blocks;
+  a.s_block = src_s_block; a.s_head = src_s_head; a.s_token = src_s_token;
+  a.c_block = sc_block; a.c_head = sc_head; a.c_token = sc_token;
+  a.d_block = dst_s_block; a.d_head = dst_s_head; a.d_token = dst_s_token;
+  a.err = err_flag;
+  // a unit is about one unrolled pass of the CTA (4 pieces of K and of V per thread)
+  const int64_t pieces = (int64_t)num_kv_heads * block_size * (head_size / 16);
+  const int64_t bpu = 4 * kThreads / pieces;
+  a.bpu = (int)(bpu < 1 ? 1 : bpu);
+  a.units_per_seq = (max_blocks_per_seq + a.bpu - 1) / a.bpu;
+  const int64_t units = num_seqs * a.units_per_seq;
+  const dim3 grid((unsigned)(units < (1 << 20) ? units : (1 << 20)));
+  auto st = static_cast<cudaStream_t>(stream);
+  int rc = 1;
+  switch (head_size) {
+    case 32: rc = va_host::launch_pdl(kv_dequant_kernel<32>, grid, kThreads, st, a); break;
+    case 64: rc = va_host::launch_pdl(kv_dequant_kernel<64>, grid, kThreads, st, a); break;
+    case 96: rc = va_host::launch_pdl(kv_dequant_kernel<96>, grid, kThreads, st, a); break;
+    case 128: rc = va_host::launch_pdl(kv_dequant_kernel<128>, grid, kThreads, st, a); break;
+  }
+  return rc ? VA_ERR_LAUNCH : va_host::launch_status();
+}

@@ -1,0 +1,634 @@
+// Single-token attention over a paged cache under a sliding window with sinks
+// (visibility rule: window.cuh), fp16 or e4m3 cache (row format: kv_q8.cuh), with the
+// write of the new row.
+//
+//   out_h = sum_j p_hj v_j / sum_j p_hj,   p_hj = 2^(scale log2(e) q_h.k_j - m_h)
+//
+// Every K/V byte of a sequence is read once per kv head and serves all query heads of
+// its group, so the kernel is bound by HBM; everything else is kept off its way:
+//   * The products run on mma.sync m16n8k16 with the KEYS as the 16 rows and the query
+//     heads as the 8 columns (S^T = K Q^T, then O^T = V^T P^T), so a group of up to 8
+//     heads fills the instruction's columns and an e4m3 cache (half the bytes per key)
+//     does not run into the FP32 pipe, as one FMA per head and value would.
+//   * The order of a contraction's terms is free, so each lane's fragment of K is made
+//     of consecutive values of a row (and of V of consecutive values of four rows): a
+//     lane copies exactly the bytes that it will feed to the tensor core with its own
+//     cp.async into its own shared-memory slots.  No lane reads another's bytes: the
+//     pipeline needs no barrier, only cp.async.wait_group.
+//   * A warp takes every 4th tile of 16 keys of its CTA's range; kStages tiles per warp
+//     are in flight.  S^T comes out of the MMA with keys in rows; P^T is wanted with keys
+//     in columns: one 8x8 transpose (movmatrix) per 8 keys.
+//   * Statistics, sums and O are fp32; P is rounded to fp16 (2^-11 of a value <= 1) for
+//     the second product.  An e4m3 code becomes fp16 exactly; the exponent of a K row
+//     scales its fp32 score, that of a V row its fp16 values (both exact).
+//   * Long contexts with few sequences are cut into ranges of tiles, one CTA each; the
+//     ranges' (O, m, l) are merged in range order by a second kernel launched as a
+//     programmatic dependent.
+//   * Keys that the query does not see are zero-filled, never read: what lies in the
+//     cache behind a sequence, before its window or in a freed block does not matter.
+#include "window.cuh"
+
+namespace {
+
+constexpr int kNW = 4;  // warps per CTA
+constexpr int kKeys = 16;
+
+template <int D, bool Q8>
+struct Shape {
+  static constexpr int ES = Q8 ? 1 : 2;                    // bytes per value
+  static constexpr int KB = (D / 4 * ES) % 16 ? 8 : 16;    // K: bytes per copy
+  static constexpr int KN = D / 4 * ES / KB;               // copies per row and lane
+  static constexpr int KE = KB / ES;                       // values per copy
+  static constexpr int VB = (D / 8 * ES) % 16 == 0 ? 16 : (D / 8 * ES) % 8 == 0 ? 8 : 4;
+  static constexpr int VN = D / 8 * ES / VB;
+  static constexpr int VE = VB / ES;
+  static constexpr int oV = 2 * KN * KB * 32;              // stage: K slots, V slots, scales
+  static constexpr int oS = oV + 4 * VN * VB * 32;
+  static constexpr int kStage = oS + (Q8 ? 128 : 0);
+  static constexpr int kStages = D * ES >= 256 ? 3 : 4;
+  static constexpr int kRing = kNW * kStages * kStage;
+};
+
+struct Args {
+  __half *out;
+  const __half *q;
+  uint8_t *kc, *vc;   // cache bytes (fp16 or e4m3)
+  uint8_t *ks, *vs;   // exponent bytes (e4m3 caches)
+  const __half *nk, *nv;
+  const int32_t *bt, *sl;
+  float *ws_acc;
+  float2 *ws_ml;
+  int32_t *err;
+  int64_t max_blocks, num_blocks, max_len;
+  int Hq, G, hg, gc, bs, window, sinks, tps, splits;
+  float scale_log2;
+  int64_t s_block, s_head, s_token, c_block, c_head, c_token;
+  int64_t q_s_token, q_s_head, o_s_token, o_s_head, n_s_token, n_s_head;
+};
+
+VA_DEVINL void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                   uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+      "{%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+VA_DEVINL uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+template <int V>
+VA_DEVINL void lds(uint32_t (&w)[V / 4], const unsigned char *p) {
+  if constexpr (V == 16) {
+    const uint4 x = *reinterpret_cast<const uint4 *>(p);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+  } else if constexpr (V == 8) {
+    const uint2 x = *reinterpret_cast<const uint2 *>(p);
+    w[0] = x.x; w[1] = x.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t *>(p);
+  }
+}
+
+// Length of a sequence, 0 when it is skipped.
+VA_DEVINL int seq_len(const Args &a, int seq, bool flag) {
+  const int L = __ldg(a.sl + seq);
+  if (L <= 0) return 0;
+  if (L > a.max_len || (L + (int64_t)a.bs - 1) / a.bs > a.max_blocks) {
+    if (flag) va::raise_flag(a.err, VA_FLAG_CTX_OVERFLOW);
+    return 0;
+  }
+  return L;
+}
+
+// The new K (threads 0..15) and V (threads 16..31) row of one kv head into the cache.
+template <int D, bool Q8>
+VA_DEVINL void write_new_row(const Args &a, int seq, int kvh, int64_t blk, int off) {
+  const int sub = threadIdx.x & 15;
+  const bool is_v = threadIdx.x & 16, on = sub * 8 < D;
+  const __half *src = (is_v ? a.nv : a.nk) + seq * a.n_s_token + kvh * a.n_s_head + sub * 8;
+  uint4 w = make_uint4(0, 0, 0, 0);
+  if (on) w = *reinterpret_cast<const uint4 *>(src);
+  const int64_t dst = blk * a.s_block + kvh * a.s_head + off * a.s_token + sub * 8;
+  uint8_t *cache = is_v ? a.vc : a.kc;
+  if constexpr (!Q8) {
+    if (on) *reinterpret_cast<uint4 *>(cache + 2 * dst) = w;
+  } else {
+    uint32_t m = va::q8_absmax2(
+        va::q8_absmax2(va::q8_absmax2(va::q8_absmax2(0, w.x), w.y), w.z), w.w);
+    m = max(m & 0xffffu, m >> 16);
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const int e = va::q8_exponent(m);
+    const float inv = va::q8_pow2(-e);
+    if (on) {
+      uint2 c;
+      c.x = va::q8_encode2(w.x, inv) | va::q8_encode2(w.y, inv) << 16;
+      c.y = va::q8_encode2(w.z, inv) | va::q8_encode2(w.w, inv) << 16;
+      *reinterpret_cast<uint2 *>(cache + dst) = c;
+    }
+    if (sub == 0)
+      (is_v ? a.vs : a.ks)[blk * a.c_block + kvh * a.c_head + off * a.c_token] =
+          (uint8_t)(e + va::kQ8ExpBias);
+  }
+}
+
+// NT: tiles of 8 query heads per warp (1 for groups of up to 8, 2 up to 16).
+template <int D, bool Q8, int NT>
+__global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
+  using S = Shape<D, Q8>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ int s_bad;
+  va::pdl_enter();
+  const int split = blockIdx.x, seq = blockIdx.z;
+  const int kvh = blockIdx.y / a.hg, head0 = kvh * a.G + (blockIdx.y - kvh * a.hg) * a.gc;
+  const int nheads = min(a.gc, (kvh + 1) * a.G - head0);
+  const int L = seq_len(a, seq, split == 0 && blockIdx.y == 0 && threadIdx.x == 0);
+  if (L == 0) return;
+  const win::Tiles tl = win::key_tiles(L - 1, L - 1, a.window, a.sinks, kKeys);
+  const int t_begin = split * a.tps, t_end = min(t_begin + a.tps, tl.count);
+  if (t_begin >= t_end) return;
+  const int nsplit = (tl.count + a.tps - 1) / a.tps;
+  const int lo = win::run_start(L - 1, a.window);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int32_t *bt = a.bt + seq * a.max_blocks;
+  if (threadIdx.x == 0) s_bad = 0;
+
+  // The CTA that reads the newest key writes it first, then reads it back with the rest.
+  if (a.nk && t_end == tl.count) {
+    const int page = (L - 1) / a.bs;
+    const int32_t blk = __ldg(bt + page);
+    if (threadIdx.x < 32 && blk >= 0 && blk < a.num_blocks)
+      write_new_row<D, Q8>(a, seq, kvh, blk, L - 1 - page * a.bs);
+  }
+
+  // Q^T fragments: columns = heads, rows in the order of the K fragments below
+  uint32_t qf[NT][D / 16][2];
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      const int e = 4 * ks, d = e / S::KE * (4 * S::KE) + t * S::KE + e % S::KE;
+      uint2 w = make_uint2(0, 0);
+      if (n * 8 + g < nheads)
+        w = __ldg(reinterpret_cast<const uint2 *>(a.q + seq * a.q_s_token +
+                                                  (int64_t)(head0 + n * 8 + g) * a.q_s_head + d));
+      qf[n][ks][0] = w.x;
+      qf[n][ks][1] = w.y;
+    }
+  __syncthreads();
+
+  // ---- copy pipeline: tile i of this warp is key tile t_begin + warp + i * kNW ----
+  const int ntiles = max(0, (t_end - t_begin - warp + kNW - 1) / kNW);
+  unsigned char *ring = smem + warp * S::kStages * S::kStage;
+  const bool one_block = a.bs % kKeys == 0;  // a tile never straddles two blocks
+  const int64_t head_off = kvh * a.s_head;
+  const int64_t c_head_off = kvh * a.c_head;
+  bool bad = false;
+  auto key_tile = [&](int i) { return win::tile_at(tl, t_begin + warp + i * kNW); };
+  // block of this lane's key (lane & 15) of tile i; -1 when the key is not visible
+  auto block_of = [&](int i) -> int32_t {
+    if (i >= ntiles) return -1;
+    const int key = key_tile(i) * kKeys + (lane & 15);
+    if (!(key < L && (key >= lo || key < a.sinks))) return -1;
+    const int32_t b = __ldg(bt + key / a.bs);
+    if (b < 0 || b >= a.num_blocks) {
+      bad = true;
+      return -1;
+    }
+    return b;
+  };
+  int32_t blk = block_of(0);
+  uint32_t sc_prev = 0;  // exponent byte of the tile copied last ...
+  unsigned char *sc_at = nullptr;  // ... and where it goes once it has arrived
+  auto put_scale = [&]() {
+    if constexpr (Q8) {
+      if (sc_at) {
+        if (lane < 16)  // K: fp32 2^e; V: fp16 2^e
+          reinterpret_cast<uint32_t *>(sc_at)[lane] = sc_prev << 23;
+        else
+          reinterpret_cast<uint16_t *>(sc_at)[lane + 16] = (uint16_t)va::q8_scale_h2(sc_prev);
+      }
+    }
+  };
+  auto copy_tile = [&](int i) {
+    put_scale();
+    sc_at = nullptr;
+    if (i < ntiles) {
+      unsigned char *st = ring + (i % S::kStages) * S::kStage;
+      const int key0 = key_tile(i) * kKeys;
+      const int off = one_block ? key0 % a.bs + (lane & 15) : (key0 + (lane & 15)) % a.bs;
+      const bool on = blk >= 0;
+      const int64_t row = on ? blk * a.s_block + head_off + off * a.s_token : 0;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {  // K rows g, g + 8
+        const int64_t rr = __shfl_sync(0xffffffffu, row, g + 8 * r);
+        const bool ro = __shfl_sync(0xffffffffu, (int)on, g + 8 * r);
+#pragma unroll
+        for (int c = 0; c < S::KN; ++c)
+          win::cp_async_zfill<S::KB>(
+              va::smem_addr(st + ((r * S::KN + c) * 32 + lane) * S::KB),
+              a.kc + (rr + c * 4 * S::KE + t * S::KE) * S::ES, ro);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {  // V rows 2t, 2t + 1, 2t + 8, 2t + 9
+        const int k = 2 * t + (r & 1) + 8 * (r >> 1);
+        const int64_t rr = __shfl_sync(0xffffffffu, row, k);
+        const bool ro = __shfl_sync(0xffffffffu, (int)on, k);
+#pragma unroll
+        for (int c = 0; c < S::VN; ++c)
+          win::cp_async_zfill<S::VB>(
+              va::smem_addr(st + S::oV + ((r * S::VN + c) * 32 + lane) * S::VB),
+              a.vc + (rr + c * 8 * S::VE + g * S::VE) * S::ES, ro);
+      }
+      if constexpr (Q8) {  // lanes 0..15: the K exponents, 16..31: V's
+        const uint8_t *p = (lane < 16 ? a.ks : a.vs) + (on ? blk * a.c_block + c_head_off +
+                                                                 off * a.c_token
+                                                           : 0);
+        sc_prev = on ? *p : va::kQ8ExpBias;
+        sc_at = st + S::oS;
+      }
+      blk = block_of(i + 1);
+    }
+    win::cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S::kStages - 1; ++i) copy_tile(i);
+
+  float m[NT][2], l[NT][2], o[NT][D / 16][4];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
+  }
+
+#pragma unroll 1
+  for (int i = 0; i < ntiles; ++i) {
+    copy_tile(i + S::kStages - 1);
+    win::cp_async_wait<S::kStages - 1>();
+    __syncwarp();  // the scales were stored by other lanes
+    const unsigned char *st = ring + (i % S::kStages) * S::kStage;
+    const int key0 = key_tile(i) * kKeys;
+    // ---- S^T = K Q^T ----
+    float s[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+    for (int c = 0; c < S::KN; ++c) {
+      uint32_t wa[S::KB / 4], wb[S::KB / 4];
+      lds<S::KB>(wa, st + (c * 32 + lane) * S::KB);
+      lds<S::KB>(wb, st + ((S::KN + c) * 32 + lane) * S::KB);
+#pragma unroll
+      for (int x = 0; x < S::KE / 4; ++x) {
+        uint32_t a0, a1, a2, a3;
+        if constexpr (Q8) {
+          a0 = va::q8_decode2(wa[x]);
+          a2 = va::q8_decode2(wa[x] >> 16);
+          a1 = va::q8_decode2(wb[x]);
+          a3 = va::q8_decode2(wb[x] >> 16);
+        } else {
+          a0 = wa[2 * x];
+          a2 = wa[2 * x + 1];
+          a1 = wb[2 * x];
+          a3 = wb[2 * x + 1];
+        }
+        const int ks = c * (S::KE / 4) + x;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma(s[n], a0, a1, a2, a3, qf[n][ks][0], qf[n][ks][1]);
+      }
+    }
+    // ---- scale, mask, online softmax (rows g, g + 8 of the tile; columns 2t, 2t + 1) ----
+    float fa = a.scale_log2, fb = a.scale_log2;
+    if constexpr (Q8) {
+      const float *f = reinterpret_cast<const float *>(st + S::oS);
+      fa *= f[g];
+      fb *= f[g + 8];
+    }
+    const int ka = key0 + g, kb = ka + 8;
+    const bool va_ = ka < L && (ka >= lo || ka < a.sinks);
+    const bool vb_ = kb < L && (kb >= lo || kb < a.sinks);
+    uint32_t pb[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      float x0 = va_ ? s[n][0] * fa : -INFINITY, x1 = va_ ? s[n][1] * fa : -INFINITY;
+      float y0 = vb_ ? s[n][2] * fb : -INFINITY, y1 = vb_ ? s[n][3] * fb : -INFINITY;
+      float m0 = fmaxf(x0, y0), m1 = fmaxf(x1, y1);
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) {
+        m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, w));
+        m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, w));
+      }
+      m0 = fmaxf(m0, m[n][0]);
+      m1 = fmaxf(m1, m[n][1]);
+      if (__any_sync(0xffffffffu, m0 != m[n][0] || m1 != m[n][1])) {
+        const float f0 = m0 == m[n][0] ? 1.f : va::fast_exp2(m[n][0] - m0);
+        const float f1 = m1 == m[n][1] ? 1.f : va::fast_exp2(m[n][1] - m1);
+        m[n][0] = m0;
+        m[n][1] = m1;
+        l[n][0] *= f0;
+        l[n][1] *= f1;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          o[n][k][0] *= f0;
+          o[n][k][1] *= f1;
+          o[n][k][2] *= f0;
+          o[n][k][3] *= f1;
+        }
+      }
+      // every tile holds a visible key, so m is finite unless a score is not
+      x0 = va::fast_exp2(x0 - m0);
+      x1 = va::fast_exp2(x1 - m1);
+      y0 = va::fast_exp2(y0 - m0);
+      y1 = va::fast_exp2(y1 - m1);
+      l[n][0] += x0 + y0;
+      l[n][1] += x1 + y1;
+      pb[n][0] = transpose8x8(va::pack_h2(x0, x1));
+      pb[n][1] = transpose8x8(va::pack_h2(y0, y1));
+    }
+    // ---- O^T += V^T P^T ----
+    uint32_t f01 = 0, f89 = 0;
+    if constexpr (Q8) {
+      const uint32_t *f = reinterpret_cast<const uint32_t *>(st + S::oS + 64);
+      f01 = f[t];
+      f89 = f[t + 4];
+    }
+#pragma unroll
+    for (int c = 0; c < S::VN; ++c) {
+      uint32_t w[4][S::VB / 4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        lds<S::VB>(w[r], st + S::oV + ((r * S::VN + c) * 32 + lane) * S::VB);
+#pragma unroll
+      for (int x = 0; x < S::VE / 2; ++x) {  // values 2x, 2x + 1 of the copy
+        uint32_t a0, a1, a2, a3;
+        if constexpr (Q8) {
+          const uint32_t sel = x & 1 ? 0x7362 : 0x5140;
+          const uint32_t u = __byte_perm(w[0][x / 2], w[1][x / 2], sel);
+          const uint32_t v = __byte_perm(w[2][x / 2], w[3][x / 2], sel);
+          a0 = va::hmul2(va::q8_decode2(u), f01);
+          a1 = va::hmul2(va::q8_decode2(u >> 16), f01);
+          a2 = va::hmul2(va::q8_decode2(v), f89);
+          a3 = va::hmul2(va::q8_decode2(v >> 16), f89);
+        } else {
+          a0 = __byte_perm(w[0][x], w[1][x], 0x5410);
+          a1 = __byte_perm(w[0][x], w[1][x], 0x7632);
+          a2 = __byte_perm(w[2][x], w[3][x], 0x5410);
+          a3 = __byte_perm(w[2][x], w[3][x], 0x7632);
+        }
+        const int k = c * (S::VE / 2) + x;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma(o[n][k], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+      }
+    }
+    __syncwarp();  // the next copy stores scales over this stage's
+  }
+  win::cp_async_wait<0>();
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int w = 4; w < 32; w <<= 1) {
+      l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], w);
+      l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], w);
+    }
+  if (bad) s_bad = 1;
+  __syncthreads();  // the ring is free: the warps' results go there
+
+  constexpr int NH = 8 * NT;
+  float *so = reinterpret_cast<float *>(smem);     // [kNW][NH][D]
+  float *sm = so + kNW * NH * D, *sl = sm + kNW * NH;  // [kNW][NH]
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int e = 2 * k + y, d = e / S::VE * (8 * S::VE) + g * S::VE + e % S::VE;
+        so[(warp * NH + n * 8 + 2 * t) * D + d] = o[n][k][2 * y];
+        so[(warp * NH + n * 8 + 2 * t + 1) * D + d] = o[n][k][2 * y + 1];
+      }
+    if (g == 0) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        sm[warp * NH + n * 8 + 2 * t + y] = m[n][y];
+        sl[warp * NH + n * 8 + 2 * t + y] = l[n][y];
+      }
+    }
+  }
+  __syncthreads();
+  const bool skip = s_bad != 0;
+  if (skip && threadIdx.x == 0) va::raise_flag(a.err, VA_FLAG_BAD_BLOCK);
+  for (int i = threadIdx.x; i < nheads * D; i += kNW * 32) {
+    const int h = i / D, d = i - h * D;
+    float M = sm[h];
+#pragma unroll
+    for (int w = 1; w < kNW; ++w) M = fmaxf(M, sm[w * NH + h]);
+    float A = 0.f, Ls = 0.f;
+#pragma unroll
+    for (int w = 0; w < kNW; ++w) {
+      // a warp without tiles has m = -inf and adds nothing
+      const float f = sm[w * NH + h] == -INFINITY ? 0.f : va::fast_exp2(sm[w * NH + h] - M);
+      A += so[(w * NH + h) * D + d] * f;
+      Ls += sl[w * NH + h] * f;
+    }
+    if (nsplit == 1) {
+      if (!skip)
+        a.out[seq * a.o_s_token + (int64_t)(head0 + h) * a.o_s_head + d] = __float2half_rn(A / Ls);
+    } else {
+      const int64_t p = ((int64_t)seq * a.Hq + head0 + h) * a.splits + split;
+      a.ws_acc[p * D + d] = A;
+      // l < 0 marks a range with an unreadable block: its sequence is left alone
+      if (d == 0) a.ws_ml[p] = make_float2(M, skip ? -1.f : Ls);
+    }
+  }
+}
+
+// Merges the ranges of the sequences that have more than one, in range order; one thread
+// per output value.
+__global__ void __launch_bounds__(256) window_decode_merge_kernel(const Args a, int D) {
+  va::pdl_enter();
+  const int seq = blockIdx.x;
+  const int L = seq_len(a, seq, false);
+  if (L == 0) return;
+  const win::Tiles tl = win::key_tiles(L - 1, L - 1, a.window, a.sinks, kKeys);
+  const int nsplit = (tl.count + a.tps - 1) / a.tps;
+  if (nsplit == 1) return;
+  const int i = blockIdx.y * 256 + threadIdx.x;
+  if (i >= a.Hq * D) return;
+  const int h = i / D, d = i - h * D;
+  const int64_t p = ((int64_t)seq * a.Hq + h) * a.splits;
+  float M = -INFINITY, A = 0.f, Ls = 0.f;
+  bool skip = false;
+  for (int s = 0; s < nsplit; ++s) {
+    const float2 v = a.ws_ml[p + s];
+    skip = skip || v.y < 0.f;
+    M = fmaxf(M, v.x);
+  }
+  if (skip) return;
+#pragma unroll 4
+  for (int s = 0; s < nsplit; ++s) {
+    const float2 v = a.ws_ml[p + s];
+    const float f = v.x == -INFINITY ? 0.f : va::fast_exp2(v.x - M);
+    A = fmaf(a.ws_acc[(p + s) * D + d], f, A);
+    Ls = fmaf(v.y, f, Ls);
+  }
+  a.out[seq * a.o_s_token + (int64_t)h * a.o_s_head + d] = __float2half_rn(A / Ls);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+struct Plan {
+  int gc, hg, tps, splits;
+  size_t o_ml, total;
+};
+
+// Head groups of up to 16; ranges so that about kTargetCtas CTAs have work, at least two
+// tiles per warp each.
+Plan make_plan(int64_t num_seqs, int Hq, int Hkv, int D, int64_t max_len, int window, int sinks) {
+  constexpr int64_t kTargetCtas = 148 * 6;
+  Plan p{};
+  const int G = Hq / Hkv;
+  p.hg = (G + 15) / 16;
+  p.gc = (G + p.hg - 1) / p.hg;
+  int64_t keys = max_len;
+  if (window > 0 && (int64_t)window + sinks < keys) keys = (int64_t)window + sinks;
+  // an unaligned run and the sinks each reach into one more tile
+  const int64_t tiles = (keys + kKeys - 1) / kKeys + 2;
+  const int64_t units = num_seqs * Hkv * p.hg;
+  int64_t splits = kTargetCtas / (units > 0 ? units : 1);
+  const int64_t most = tiles / (2 * kNW);
+  if (splits > most) splits = most;
+  if (splits < 1) splits = 1;
+  const int64_t tps = (tiles + splits - 1) / splits;
+  p.tps = (int)tps;
+  p.splits = (int)((tiles + tps - 1) / tps);
+  if (p.splits > 1) {
+    const size_t parts = (size_t)num_seqs * Hq * p.splits;
+    p.o_ml = (parts * D * 4 + 255) & ~size_t(255);
+    p.total = p.o_ml + ((parts * 8 + 255) & ~size_t(255));
+  }
+  return p;
+}
+
+template <int D, bool Q8, int NT>
+int launch_t(const Args &a, dim3 grid, cudaStream_t st) {
+  constexpr int merge = kNW * 8 * NT * (D + 2) * 4;
+  constexpr int smem = Shape<D, Q8>::kRing > merge ? Shape<D, Q8>::kRing : merge;
+  if (smem > 48 * 1024) {
+    // the opt-in is per device; setting it again is cheap and needs no state
+    if (cudaFuncSetAttribute(window_decode_kernel<D, Q8, NT>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return VA_ERR_LAUNCH;
+  }
+  if (va_host::launch_pdl_smem(window_decode_kernel<D, Q8, NT>, grid, kNW * 32, smem, st, a))
+    return VA_ERR_LAUNCH;
+  if (a.splits > 1 &&
+      va_host::launch_pdl(window_decode_merge_kernel,
+                          dim3(grid.z, (unsigned)((a.Hq * D + 255) / 256)), 256, st, a, D))
+    return VA_ERR_LAUNCH;
+  return va_host::launch_status();
+}
+
+template <int D>
+int launch_d(bool q8, const Args &a, dim3 grid, cudaStream_t st) {
+  if (q8) return a.gc <= 8 ? launch_t<D, true, 1>(a, grid, st) : launch_t<D, true, 2>(a, grid, st);
+  return a.gc <= 8 ? launch_t<D, false, 1>(a, grid, st) : launch_t<D, false, 2>(a, grid, st);
+}
+
+}  // namespace
+
+extern "C" size_t va_window_decode_workspace_size(int64_t num_seqs, int num_query_heads,
+                                                  int num_kv_heads, int head_size,
+                                                  int64_t max_seq_len, int window,
+                                                  int sink_tokens) {
+  if (num_seqs <= 0 || num_kv_heads <= 0 || num_query_heads <= 0 || head_size <= 0 ||
+      num_query_heads % num_kv_heads || max_seq_len <= 0 || sink_tokens < 0)
+    return 0;
+  return make_plan(num_seqs, num_query_heads, num_kv_heads, head_size, max_seq_len, window,
+                   sink_tokens)
+      .total;
+}
+
+extern "C" int va_window_decode(void *out, const void *q, void *k_cache, void *v_cache,
+                                void *k_scale, void *v_scale, int kv_e4m3,
+                                const int32_t *block_table, const int32_t *seq_lens,
+                                const void *new_k, const void *new_v, int64_t num_seqs,
+                                int num_query_heads, int num_kv_heads, int head_size,
+                                int block_size, int64_t max_blocks_per_seq, int64_t max_seq_len,
+                                int64_t num_blocks, float scale, int window, int sink_tokens,
+                                int64_t s_block, int64_t s_head, int64_t s_token,
+                                int64_t sc_block, int64_t sc_head, int64_t sc_token,
+                                int64_t q_s_token, int64_t q_s_head, int64_t o_s_token,
+                                int64_t o_s_head, int64_t new_s_token, int64_t new_s_head,
+                                void *workspace, size_t workspace_bytes, int32_t *err_flag,
+                                void *stream) {
+  if (num_seqs < 0 || max_seq_len < 0 || num_blocks < 0 || max_blocks_per_seq < 0 ||
+      sink_tokens < 0 || !win::scale_ok(scale))
+    return VA_ERR_INVALID_ARG;
+  if (num_kv_heads <= 0 || num_query_heads <= 0 || num_query_heads % num_kv_heads ||
+      block_size <= 0)
+    return VA_ERR_INVALID_ARG;
+  if (num_seqs == 0 || max_seq_len == 0) return VA_OK;
+  if (!out || !q || !k_cache || !v_cache || !block_table || !seq_lens ||
+      (kv_e4m3 && (!k_scale || !v_scale)) || (new_k == nullptr) != (new_v == nullptr))
+    return VA_ERR_INVALID_ARG;
+  if (!win::head_size_ok(head_size) || num_seqs > 65535) return VA_ERR_UNSUPPORTED;
+  if (max_seq_len > INT32_MAX / 2) return VA_ERR_UNSUPPORTED;
+  if (!va_host::aligned16(k_cache) || !va_host::aligned16(v_cache) ||
+      !win::strides_ok(kv_e4m3, s_block, s_head, s_token) ||
+      !win::rows_ok(q, q_s_token, q_s_head) || (reinterpret_cast<uintptr_t>(out) & 1))
+    return VA_ERR_INVALID_ARG;
+  if (new_k && (!win::rows_ok(new_k, new_s_token, new_s_head) || !va_host::aligned16(new_v)))
+    return VA_ERR_INVALID_ARG;
+  const Plan p = make_plan(num_seqs, num_query_heads, num_kv_heads, head_size, max_seq_len,
+                           window, sink_tokens);
+  if ((int64_t)num_kv_heads * p.hg > 65535) return VA_ERR_UNSUPPORTED;
+  if (p.total && (!workspace || workspace_bytes < p.total || !va_host::aligned16(workspace)))
+    return VA_ERR_WORKSPACE;
+  Args a{};
+  a.out = static_cast<__half *>(out);
+  a.q = static_cast<const __half *>(q);
+  a.kc = static_cast<uint8_t *>(k_cache);
+  a.vc = static_cast<uint8_t *>(v_cache);
+  a.ks = static_cast<uint8_t *>(k_scale);
+  a.vs = static_cast<uint8_t *>(v_scale);
+  a.nk = static_cast<const __half *>(new_k);
+  a.nv = static_cast<const __half *>(new_v);
+  a.bt = block_table;
+  a.sl = seq_lens;
+  a.ws_acc = static_cast<float *>(workspace);
+  a.ws_ml = p.total ? reinterpret_cast<float2 *>(static_cast<unsigned char *>(workspace) + p.o_ml)
+                    : nullptr;
+  a.err = err_flag;
+  a.max_blocks = max_blocks_per_seq;
+  a.num_blocks = num_blocks;
+  a.max_len = max_seq_len;
+  a.Hq = num_query_heads;
+  a.G = num_query_heads / num_kv_heads;
+  a.hg = p.hg;
+  a.gc = p.gc;
+  a.bs = block_size;
+  a.window = window;
+  a.sinks = sink_tokens;
+  a.tps = p.tps;
+  a.splits = p.splits;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.s_block = s_block; a.s_head = s_head; a.s_token = s_token;
+  a.c_block = sc_block; a.c_head = sc_head; a.c_token = sc_token;
+  a.q_s_token = q_s_token; a.q_s_head = q_s_head;
+  a.o_s_token = o_s_token; a.o_s_head = o_s_head;
+  a.n_s_token = new_s_token; a.n_s_head = new_s_head;
+  const dim3 grid((unsigned)p.splits, (unsigned)(num_kv_heads * p.hg), (unsigned)num_seqs);
+  auto st = static_cast<cudaStream_t>(stream);
+  switch (head_size) {
+    case 32: return launch_d<32>(kv_e4m3 != 0, a, grid, st);
+    case 64: return launch_d<64>(kv_e4m3 != 0, a, grid, st);
+    case 96: return launch_d<96>(kv_e4m3 != 0, a, grid, st);
+    case 128: return launch_d<128>(kv_e4m3 != 0, a, grid, st);
+  }
+  return VA_ERR_UNSUPPORTED;
+}

@@ -395,3 +395,197 @@ def kv_sync_blocks(src_k, src_v, dst_k, dst_v, block_table, seq_lens, src_layout
         block_table.data_ptr(), seq_lens.data_ptr(), seq_lens.numel(), block_table.shape[1],
         s.num_kv_heads, s.head_size, s.block_size, s.num_blocks, s.s_block, s.s_head, s.s_token,
         d.s_block, d.s_head, d.s_token, _stream(dev)), "va_kv_sync_blocks")
+
+
+# ---------------------------------------------------------------------------
+# 8-bit KV cache and windowed attention
+# ---------------------------------------------------------------------------
+def _launch(dev: int, name: str, *args) -> None:
+    """Call a C entry point with device ``dev`` current (the library launches on the
+    current device; the arguments end with a stream of ``dev``)."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == dev:
+        status = fn(*args)
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args)
+    if status:
+        _lib.check(status, name)
+
+
+def _on(dev: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, the call runs on {dev}")
+
+
+def call_workspace(device: int, kind: str, nbytes: int,
+                   stream: torch.cuda.Stream | None = None) -> torch.Tensor | None:
+    """Scratch of at least ``nbytes`` for one call on ``stream`` (default: current).
+
+    Eager calls share :func:`workspace`'s buffer of their stream.  A call that is being
+    captured gets its own from the graph's memory pool: two captured graphs may replay
+    at the same time on different streams, so they must not share one."""
+    if not nbytes:
+        return None
+    if torch.cuda.is_current_stream_capturing():
+        st = torch.cuda.current_stream(device) if stream is None else stream
+        with torch.cuda.stream(st):
+            return torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
+    return workspace(device, kind, nbytes, stream)
+
+
+def _window_cache(k_cache, v_cache, k_scale, v_scale, layout):
+    """(kv_e4m3, geometry, exponent strides in (block, head, token) order) of a cache pair
+    that is fp16 (no scales) or e4m3 with its exponent bytes."""
+    q8 = k_cache.dtype == torch.float8_e4m3fn
+    if not q8 and k_cache.dtype != torch.float16:
+        raise TypeError(f"KV cache must be float16 or float8_e4m3fn, got {k_cache.dtype}")
+    if layout not in ("hnd", "nhd"):
+        raise ValueError(f"unknown cache layout {layout!r}")
+    st = k_cache.stride()
+    if k_cache.dim() != 4 or (st[3] != 1 and k_cache.shape[3] > 1):
+        raise ValueError("KV cache must be 4-D with a contiguous head_size axis")
+    if v_cache.dtype != k_cache.dtype or v_cache.shape != k_cache.shape or v_cache.stride() != st:
+        raise ValueError("K and V caches differ in type, shape or strides")
+    if not q8:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("k_scale / v_scale belong to an e4m3 cache")
+        sc = (0, 0, 0)
+    else:
+        if k_scale is None or v_scale is None:
+            raise ValueError("an e4m3 cache needs k_scale and v_scale")
+        for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if t.dtype != torch.uint8:
+                raise TypeError(f"{n} must be uint8 (exponent + 127), got {t.dtype}")
+            if t.shape != k_cache.shape[:3]:
+                raise ValueError(f"{n} must have the cache's first three dimensions "
+                                 f"{tuple(k_cache.shape[:3])}, got {tuple(t.shape)}")
+        sc = k_scale.stride()
+        if v_scale.stride() != sc:
+            raise ValueError("k_scale and v_scale differ in strides")
+    if layout == "hnd":
+        nb, h, bs, d = k_cache.shape
+        return q8, CacheGeom(nb, h, bs, d, st[0], st[1], st[2]), sc
+    nb, bs, h, d = k_cache.shape
+    return q8, CacheGeom(nb, h, bs, d, st[0], st[2], st[1]), (sc[0], sc[2], sc[1])
+
+
+def _new_rows(new_k, new_v, g: CacheGeom, rows: int):
+    st = _rows3(new_k, "new_k")
+    if new_v is None or _rows3(new_v, "new_v") != st or new_k.shape != new_v.shape:
+        raise ValueError("new_k and new_v differ in shape or strides")
+    if new_k.shape[1:] != (g.num_kv_heads, g.head_size) or new_k.shape[0] < rows:
+        raise ValueError(f"new_k / new_v must be [{rows}, {g.num_kv_heads}, {g.head_size}], "
+                         f"got {tuple(new_k.shape)}")
+    return st
+
+
+def _table(block_table, seqs: int) -> int:
+    """Blocks per sequence of a block table with at least ``seqs`` rows."""
+    _i32(block_table, "block_table")
+    if block_table.dim() != 2 or block_table.shape[0] < seqs:
+        raise ValueError(f"block_table must be [>= {seqs}, max_blocks], "
+                         f"got {tuple(block_table.shape)}")
+    return block_table.shape[1]
+
+
+def kv_quant_write_slots(k_cache, v_cache, k_scale, v_scale, new_k, new_v, slot_mapping,
+                         layout="hnd"):
+    """Quantise rows ``new_k/new_v`` [T, Hkv, D] and scatter them into an e4m3 cache by slot.
+
+    ``k_cache/v_cache`` are float8_e4m3fn in the fp16 cache's layouts; ``k_scale/v_scale``
+    uint8 of the same first three dimensions hold the exponent (+127) of each row: a row
+    stands for ``codes * 2 ** (scale - 127)``.  Slot -1 is skipped; live slots must be
+    distinct."""
+    dev = _dev_index(k_cache)
+    q8, g, sc = _window_cache(k_cache, v_cache, k_scale, v_scale, layout)
+    if not q8:
+        raise TypeError("kv_quant_write_slots writes a float8_e4m3fn cache")
+    if slot_mapping.dtype not in (torch.int32, torch.int64) or not slot_mapping.is_contiguous():
+        raise TypeError("slot_mapping must be a contiguous int32 or int64 tensor")
+    T = new_k.shape[0]
+    n_st, n_sh = _new_rows(new_k, new_v, g, T)
+    if slot_mapping.numel() < T:
+        raise ValueError("slot_mapping shorter than the number of tokens")
+    _on(k_cache.device, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, new_k=new_k,
+        new_v=new_v, slot_mapping=slot_mapping)
+    _launch(dev, "va_kv_quant_write_slots", k_cache.data_ptr(), v_cache.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), new_k.data_ptr(), new_v.data_ptr(),
+            slot_mapping.data_ptr(), int(slot_mapping.dtype == torch.int64), T, g.num_kv_heads,
+            g.head_size, g.block_size, g.num_blocks, g.s_block, g.s_head, g.s_token, *sc, n_st,
+            n_sh, err_flag(dev).data_ptr(), _stream(dev))
+
+
+def kv_dequant_blocks(src_k, src_v, k_scale, v_scale, dst_k, dst_v, block_table, seq_lens,
+                      dst_block_table=None, src_layout="hnd", dst_layout="hnd"):
+    """Read the active rows of every sequence of an e4m3 cache back into an fp16 cache
+    (exactly: every stored value is an fp16 value).
+
+    Block ``block_table[s, i]`` of the source goes to ``dst_block_table[s, i]`` (default:
+    the same id) of the destination; rows past a sequence's end stay as they are."""
+    dev = _dev_index(src_k)
+    q8, s, sc = _window_cache(src_k, src_v, k_scale, v_scale, src_layout)
+    if not q8:
+        raise TypeError("kv_dequant_blocks reads a float8_e4m3fn cache")
+    d = cache_geom(dst_k, dst_layout)
+    if cache_geom(dst_v, dst_layout) != d:
+        raise ValueError("K and V caches differ in shape or strides")
+    if (s.num_kv_heads, s.block_size, s.head_size) != (d.num_kv_heads, d.block_size, d.head_size):
+        raise ValueError("source and destination caches differ in geometry")
+    _i32(seq_lens, "seq_lens")
+    B = seq_lens.numel()
+    mb = _table(block_table, B)
+    if dst_block_table is not None:
+        _i32(dst_block_table, "dst_block_table")
+        if dst_block_table.shape != block_table.shape:
+            raise ValueError("dst_block_table and block_table differ in shape")
+    _on(src_k.device, src_v=src_v, k_scale=k_scale, v_scale=v_scale, dst_k=dst_k, dst_v=dst_v,
+        block_table=block_table, seq_lens=seq_lens, dst_block_table=dst_block_table)
+    _launch(dev, "va_kv_dequant_blocks", src_k.data_ptr(), src_v.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), dst_k.data_ptr(), dst_v.data_ptr(), block_table.data_ptr(),
+            _ptr(dst_block_table), seq_lens.data_ptr(), B, mb, s.num_kv_heads, s.head_size,
+            s.block_size, s.num_blocks, d.num_blocks, s.s_block, s.s_head, s.s_token, *sc,
+            d.s_block, d.s_head, d.s_token, err_flag(dev).data_ptr(), _stream(dev))
+
+
+def paged_window_decode(out, q, k_cache, v_cache, block_table, seq_lens, *, scale, max_seq_len,
+                        window=0, sink_tokens=0, k_scale=None, v_scale=None, new_k=None,
+                        new_v=None, layout="hnd", num_seqs=None):
+    """Decode attention under a sliding window with sinks, over an fp16 or e4m3 cache.
+
+    The query of sequence i sits at position ``seq_lens[i] - 1`` and sees the last
+    ``window`` positions (0: all) and the first ``sink_tokens``.  With ``new_k/new_v``
+    [B, Hkv, D] the new row is written first (quantised for an e4m3 cache).  out/q
+    [B, Hq, D]; ``max_seq_len`` >= every seq_len; ``scale`` > 0."""
+    dev = _dev_index(q)
+    q8, g, sc = _window_cache(k_cache, v_cache, k_scale, v_scale, layout)
+    q_st, q_sh = _rows3(q, "q")
+    o_st, o_sh = _rows3(out, "out")
+    _i32(seq_lens, "seq_lens")
+    B = q.shape[0] if num_seqs is None else num_seqs
+    Hq, D = q.shape[1], q.shape[2]
+    if D != g.head_size:
+        raise ValueError(f"q head_size {D} != cache head_size {g.head_size}")
+    if out.shape[0] < B or q.shape[0] < B or out.shape[1:] != q.shape[1:]:
+        raise ValueError("out and q differ in shape, or hold fewer rows than num_seqs")
+    if seq_lens.numel() < B:
+        raise ValueError("seq_lens shorter than the number of sequences")
+    mb = _table(block_table, B)
+    n_st = n_sh = 0
+    if new_k is not None or new_v is not None:
+        if new_k is None:
+            raise ValueError("new_k and new_v go together")
+        n_st, n_sh = _new_rows(new_k, new_v, g, B)
+    _on(q.device, out=out, k_cache=k_cache, v_cache=v_cache, block_table=block_table,
+        seq_lens=seq_lens, k_scale=k_scale, v_scale=v_scale, new_k=new_k, new_v=new_v)
+    window = max(int(window or 0), 0)
+    nbytes = _lib.load().va_window_decode_workspace_size(B, Hq, g.num_kv_heads, D, max_seq_len,
+                                                         window, sink_tokens)
+    ws = call_workspace(dev, "window_decode", nbytes)
+    _launch(dev, "va_window_decode", out.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), int(q8), block_table.data_ptr(),
+            seq_lens.data_ptr(), _ptr(new_k), _ptr(new_v), B, Hq, g.num_kv_heads, D,
+            g.block_size, mb, max_seq_len, g.num_blocks, float(scale), window, sink_tokens,
+            g.s_block, g.s_head, g.s_token, *sc, q_st, q_sh, o_st, o_sh, n_st, n_sh, _ptr(ws),
+            nbytes, err_flag(dev).data_ptr(), _stream(dev))
