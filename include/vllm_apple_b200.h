@@ -289,6 +289,28 @@ VA_API int va_window_decode(void *out, const void *q, void *k_cache, void *v_cac
                             int64_t new_s_token, int64_t new_s_head, void *workspace,
                             size_t workspace_bytes, int32_t *err_flag, void *stream);
 
+/* Causal attention of chunks of new tokens over their visible keys; the cache
+ * (fp16, or e4m3 with kv_e4m3 = 1) already holds the new tokens' rows.  Tokens
+ * query_start_loc[s] .. query_start_loc[s+1]-1 (int32 [num_seqs+1], ascending,
+ * inside [0, num_tokens]) are the last ones of sequence s: token t sits at
+ * position seq_lens[s] - (query_start_loc[s+1] - t).  Tokens of no sequence and
+ * tokens with a negative position are left as they are; a sequence longer than
+ * the block table or with tokens past num_tokens is flagged and left as it is,
+ * and so is a token that sees a key in a block outside the cache.  Rows of out,
+ * q and the cache start on 16-byte boundaries; at most 128 query heads per kv
+ * head; any block_size; scale positive and finite.  No workspace. */
+VA_API int va_window_prefill(void *out, const void *q, const void *k_cache, const void *v_cache,
+                             const void *k_scale, const void *v_scale, int kv_e4m3,
+                             const int32_t *block_table, const int32_t *query_start_loc,
+                             const int32_t *seq_lens, int64_t num_tokens, int64_t num_seqs,
+                             int num_query_heads, int num_kv_heads, int head_size,
+                             int block_size, int64_t max_blocks_per_seq, int64_t num_blocks,
+                             float scale, int window, int sink_tokens, int64_t s_block,
+                             int64_t s_head, int64_t s_token, int64_t sc_block, int64_t sc_head,
+                             int64_t sc_token, int64_t q_s_token, int64_t q_s_head,
+                             int64_t o_s_token, int64_t o_s_head, int32_t *err_flag,
+                             void *stream);
+
 /* ---------------------------------------------------------------------------
  * Step-level ops around the attention call
  * ------------------------------------------------------------------------- */

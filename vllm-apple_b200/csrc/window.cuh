@@ -8,6 +8,8 @@
 // read, so their block-table entries may hold anything (a freed block, -1).
 #pragma once
 
+#include <atomic>
+
 #include "kv_q8.cuh"
 
 namespace win {
@@ -61,6 +63,22 @@ inline bool rows_ok(const void *p, int64_t s_token, int64_t s_head) {
   return va_host::aligned16(p) && s_token % 8 == 0 && s_head % 8 == 0;
 }
 inline bool head_size_ok(int D) { return D == 32 || D == 64 || D == 96 || D == 128; }
+// Positions stay below INT32_MAX / 2, so a window past that is none.
+inline int window_of(int window) { return window > 0 && window < INT32_MAX / 2 ? window : 0; }
+// Opts a kernel in to `bytes` of dynamic shared memory, once per device (bit d of `done`;
+// two threads setting it at once is harmless).
+template <typename K>
+bool allow_smem(K kernel, int bytes, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+      cudaSuccess)
+    return false;
+  done.fetch_or(bit, std::memory_order_release);
+  return true;
+}
 inline bool scale_ok(float s) { return s > 0.f && s <= 3.402823466e38f; }
 
 }  // namespace win

@@ -518,12 +518,8 @@ template <int D, bool Q8, int NT>
 int launch_t(const Args &a, dim3 grid, cudaStream_t st) {
   constexpr int merge = kNW * 8 * NT * (D + 2) * 4;
   constexpr int smem = Shape<D, Q8>::kRing > merge ? Shape<D, Q8>::kRing : merge;
-  if (smem > 48 * 1024) {
-    // the opt-in is per device; setting it again is cheap and needs no state
-    if (cudaFuncSetAttribute(window_decode_kernel<D, Q8, NT>,
-                             cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-      return VA_ERR_LAUNCH;
-  }
+  static std::atomic<uint64_t> done{0};
+  if (!win::allow_smem(window_decode_kernel<D, Q8, NT>, smem, done)) return VA_ERR_LAUNCH;
   if (va_host::launch_pdl_smem(window_decode_kernel<D, Q8, NT>, grid, kNW * 32, smem, st, a))
     return VA_ERR_LAUNCH;
   if (a.splits > 1 &&
@@ -612,7 +608,7 @@ extern "C" int va_window_decode(void *out, const void *q, void *k_cache, void *v
   a.hg = p.hg;
   a.gc = p.gc;
   a.bs = block_size;
-  a.window = window;
+  a.window = win::window_of(window);
   a.sinks = sink_tokens;
   a.tps = p.tps;
   a.splits = p.splits;

@@ -71,6 +71,8 @@ SIGNATURES = {
     "va_window_decode": (c_int, [P, P, P, P, P, P, c_int, P, P, P, P, I64, c_int, c_int, c_int,
                                  c_int, I64, I64, I64, c_float, c_int, c_int, *[I64] * 12, P,
                                  c_size_t, P, P]),
+    "va_window_prefill": (c_int, [P, P, P, P, P, P, c_int, P, P, P, I64, I64, c_int, c_int, c_int,
+                                  c_int, I64, I64, c_float, c_int, c_int, *[I64] * 10, P, P]),
     "va_rope_kv_write_slots": (c_int, [P, P, P, P, P, P, P, P, P, c_int, I64, c_int, c_int, c_int,
                                        c_int, I64, I64, I64, I64, I64, I64, I64, I64, P, P]),
     "va_build_prefill_metadata": (c_int, [P, P, P, I64, I64, I64, I64, c_int, P, P, P, P]),

@@ -589,3 +589,38 @@ def paged_window_decode(out, q, k_cache, v_cache, block_table, seq_lens, *, scal
             g.block_size, mb, max_seq_len, g.num_blocks, float(scale), window, sink_tokens,
             g.s_block, g.s_head, g.s_token, *sc, q_st, q_sh, o_st, o_sh, n_st, n_sh, _ptr(ws),
             nbytes, err_flag(dev).data_ptr(), _stream(dev))
+
+
+def paged_window_prefill(out, q, k_cache, v_cache, block_table, query_start_loc, seq_lens, *,
+                         scale, window=0, sink_tokens=0, k_scale=None, v_scale=None,
+                         layout="hnd", num_seqs=None):
+    """Causal attention of chunks of new tokens under a sliding window with sinks, over an
+    fp16 or e4m3 cache that already holds the new tokens' rows.
+
+    Tokens ``query_start_loc[s] .. query_start_loc[s + 1] - 1`` of out/q [T, Hq, D] are the
+    last ones of sequence s (of length ``seq_lens[s]``); each sees itself, the ``window - 1``
+    positions before it (0: all) and the first ``sink_tokens``.  Rows of no sequence stay as
+    they are."""
+    dev = _dev_index(q)
+    q8, g, sc = _window_cache(k_cache, v_cache, k_scale, v_scale, layout)
+    q_st, q_sh = _rows3(q, "q")
+    o_st, o_sh = _rows3(out, "out")
+    _i32(query_start_loc, "query_start_loc")
+    _i32(seq_lens, "seq_lens")
+    T, Hq, D = q.shape
+    S = query_start_loc.numel() - 1 if num_seqs is None else num_seqs
+    if D != g.head_size:
+        raise ValueError(f"q head_size {D} != cache head_size {g.head_size}")
+    if out.shape != q.shape:
+        raise ValueError("out and q differ in shape")
+    if S < 0 or query_start_loc.numel() < S + 1 or seq_lens.numel() < S:
+        raise ValueError("query_start_loc / seq_lens shorter than the number of sequences")
+    mb = _table(block_table, S)
+    _on(q.device, out=out, k_cache=k_cache, v_cache=v_cache, block_table=block_table,
+        query_start_loc=query_start_loc, seq_lens=seq_lens, k_scale=k_scale, v_scale=v_scale)
+    _launch(dev, "va_window_prefill", out.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), int(q8), block_table.data_ptr(),
+            query_start_loc.data_ptr(), seq_lens.data_ptr(), T, S, Hq, g.num_kv_heads, D,
+            g.block_size, mb, g.num_blocks, float(scale), max(int(window or 0), 0), sink_tokens,
+            g.s_block, g.s_head, g.s_token, *sc, q_st, q_sh, o_st, o_sh,
+            err_flag(dev).data_ptr(), _stream(dev))
