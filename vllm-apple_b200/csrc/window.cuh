@@ -34,6 +34,30 @@ VA_DEVINL Tiles key_tiles(int first, int last, int window, int sinks, int size) 
 }
 VA_DEVINL int tile_at(const Tiles &t, int i) { return i < t.sinks ? i : t.start + i - t.sinks; }
 
+// Division of keys (0 <= n < 2^31) by a block size that is only known at launch, as one
+// multiplication: m = ceil(2^(32 + sh) / d) with 2^sh the power of two that is not below
+// d leaves a remainder too small to matter for n < 2^31.
+struct FastDiv {
+  uint32_t d, m, sh;
+  VA_DEVINL int div(int n) const {
+    if (d == 1) return n;
+    return (int)(__umulhi((uint32_t)n, m) >> sh);
+  }
+  VA_DEVINL int mod(int n) const { return n - div(n) * (int)d; }
+};
+inline FastDiv fast_div(int d) {
+  FastDiv f{};
+  f.d = (uint32_t)d;
+  if (d > 1) {
+    // sh = ceil(log2 d) - 1 keeps m in 32 bits
+    uint32_t sh = 0;
+    while ((uint64_t(2) << sh) < (uint64_t)d) ++sh;
+    f.sh = sh;
+    f.m = (uint32_t)(((uint64_t(1) << (32 + sh)) + d - 1) / d);
+  }
+  return f;
+}
+
 // Asynchronous copy of V bytes, or V zero bytes where `on` is false (the source is not
 // read then).
 template <int V>
@@ -45,6 +69,14 @@ VA_DEVINL void cp_async_zfill(uint32_t dst, const void *src, bool on) {
   else
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(V),
                  "r"(n)
+                 : "memory");
+}
+template <int V>
+VA_DEVINL void cp_async(uint32_t dst, const void *src) {
+  if constexpr (V == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(V)
                  : "memory");
 }
 VA_DEVINL void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }

@@ -10,11 +10,11 @@
 //     heads as the 8 columns (S^T = K Q^T, then O^T = V^T P^T), so a group of up to 8
 //     heads fills the instruction's columns and an e4m3 cache (half the bytes per key)
 //     does not run into the FP32 pipe, as one FMA per head and value would.
-//   * The order of a contraction's terms is free, so each lane's fragment of K is made
-//     of consecutive values of a row (and of V of consecutive values of four rows): a
-//     lane copies exactly the bytes that it will feed to the tensor core with its own
-//     cp.async into its own shared-memory slots.  No lane reads another's bytes: the
-//     pipeline needs no barrier, only cp.async.wait_group.
+//   * The order of a contraction's terms is free, so a lane's fragments of K are consecutive
+//     values of a row, and those of V consecutive values of four rows: 16-byte reads.  The
+//     rows come in by cp.async, 16 bytes a lane and whole 128-byte lines a request (with
+//     requests of 64 bytes, a fragment's own share of a row, the L2 limited the kernel), into
+//     a ring that belongs to the warp alone: no barrier, only cp.async.wait_group.
 //   * A warp takes every 4th tile of 16 keys of its CTA's range; kStages tiles per warp
 //     are in flight.  S^T comes out of the MMA with keys in rows; P^T is wanted with keys
 //     in columns: one 8x8 transpose (movmatrix) per 8 keys.
@@ -36,16 +36,28 @@ constexpr int kKeys = 16;
 template <int D, bool Q8>
 struct Shape {
   static constexpr int ES = Q8 ? 1 : 2;                    // bytes per value
-  static constexpr int KB = (D / 4 * ES) % 16 ? 8 : 16;    // K: bytes per copy
-  static constexpr int KN = D / 4 * ES / KB;               // copies per row and lane
-  static constexpr int KE = KB / ES;                       // values per copy
+  static constexpr int KB = (D / 4 * ES) % 16 ? 8 : 16;    // K: bytes per read
+  static constexpr int KN = D / 4 * ES / KB;               // reads per row and lane
+  static constexpr int KE = KB / ES;                       // values per read
   static constexpr int VB = (D / 8 * ES) % 16 == 0 ? 16 : (D / 8 * ES) % 8 == 0 ? 8 : 4;
   static constexpr int VN = D / 8 * ES / VB;
   static constexpr int VE = VB / ES;
-  static constexpr int oV = 2 * KN * KB * 32;              // stage: K slots, V slots, scales
-  static constexpr int oS = oV + 4 * VN * VB * 32;
+  static constexpr int RB = D * ES;                        // bytes of a row
+  static constexpr int P = RB / 16;                        // 16-byte pieces of a row
+  static constexpr int oV = kKeys * RB;                    // stage: K rows, V rows, exponents
+  static constexpr int oS = 2 * kKeys * RB;
+  // The rows of a stage lie one after the other, their pieces exchanged inside 128-byte
+  // lines so that the fragment reads below hit every bank once (row sizes 32 to 256; the
+  // rows of 96 and 192 bytes stay as they are).
+  static VA_DEVINL int k_swz(int r) { return RB % 128 == 0 ? (r & 1) << 6 : 0; }
+  static VA_DEVINL int v_swz(int r) {
+    return RB == 32 ? (r >> 2 & 1) << 5 : RB % 64 == 0 && RB != 192 ? (r >> 1 & 3) << 5 : 0;
+  }
   static constexpr int kStage = oS + (Q8 ? 128 : 0);
-  static constexpr int kStages = D * ES >= 256 ? 3 : 4;
+  // tiles per pass: an e4m3 tile is half the bytes, so two share a pass's reductions
+  static constexpr int KT = Q8 ? 2 : 1;
+  static constexpr int kStages = D * ES >= 256 ? 3 : 4;  // a multiple of KT
+  static constexpr int kHead = D + 4;  // floats of a head's row in the warps' merge
   static constexpr int kRing = kNW * kStages * kStage;
 };
 
@@ -60,7 +72,8 @@ struct Args {
   float2 *ws_ml;
   int32_t *err;
   int64_t max_blocks, num_blocks, max_len;
-  int Hq, G, hg, gc, bs, window, sinks, tps, splits;
+  int Hq, G, hg, gc, window, sinks, tps, splits;
+  win::FastDiv bs;
   float scale_log2;
   int64_t s_block, s_head, s_token, c_block, c_head, c_token;
   int64_t q_s_token, q_s_head, o_s_token, o_s_head, n_s_token, n_s_head;
@@ -96,7 +109,7 @@ VA_DEVINL void lds(uint32_t (&w)[V / 4], const unsigned char *p) {
 VA_DEVINL int seq_len(const Args &a, int seq, bool flag) {
   const int L = __ldg(a.sl + seq);
   if (L <= 0) return 0;
-  if (L > a.max_len || (L + (int64_t)a.bs - 1) / a.bs > a.max_blocks) {
+  if (L > a.max_len || a.bs.div(L - 1) >= a.max_blocks) {
     if (flag) va::raise_flag(a.err, VA_FLAG_CTX_OVERFLOW);
     return 0;
   }
@@ -139,7 +152,7 @@ VA_DEVINL void write_new_row(const Args &a, int seq, int kvh, int64_t blk, int o
 template <int D, bool Q8, int NT>
 __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
   using S = Shape<D, Q8>;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int s_bad;
   va::pdl_enter();
   const int split = blockIdx.x, seq = blockIdx.z;
@@ -158,10 +171,10 @@ __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
 
   // The CTA that reads the newest key writes it first, then reads it back with the rest.
   if (a.nk && t_end == tl.count) {
-    const int page = (L - 1) / a.bs;
+    const int page = a.bs.div(L - 1);
     const int32_t blk = __ldg(bt + page);
     if (threadIdx.x < 32 && blk >= 0 && blk < a.num_blocks)
-      write_new_row<D, Q8>(a, seq, kvh, blk, L - 1 - page * a.bs);
+      write_new_row<D, Q8>(a, seq, kvh, blk, L - 1 - page * (int)a.bs.d);
   }
 
   // Q^T fragments: columns = heads, rows in the order of the K fragments below
@@ -181,81 +194,101 @@ __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
   __syncthreads();
 
   // ---- copy pipeline: tile i of this warp is key tile t_begin + warp + i * kNW ----
+  constexpr int KT = S::KT, R = S::kStages;
   const int ntiles = max(0, (t_end - t_begin - warp + kNW - 1) / kNW);
-  unsigned char *ring = smem + warp * S::kStages * S::kStage;
-  const bool one_block = a.bs % kKeys == 0;  // a tile never straddles two blocks
-  const int64_t head_off = kvh * a.s_head;
-  const int64_t c_head_off = kvh * a.c_head;
+  const int npass = (ntiles + KT - 1) / KT;  // tiles past ntiles are zeros
+  unsigned char *ring = smem + warp * R * S::kStage;
+  const bool one_block = a.bs.d % kKeys == 0;  // a tile never straddles two blocks
+  // this lane's pieces lane, lane + 32, ... of a tile, in row order
+  const int64_t tok = a.s_token * S::ES;
+  const uint8_t *k_head = a.kc + kvh * a.s_head * S::ES, *v_head = a.vc + kvh * a.s_head * S::ES;
+  const uint8_t *s_lane = Q8 ? (lane < 16 ? a.ks : a.vs) + kvh * a.c_head : nullptr;
   bool bad = false;
   auto key_tile = [&](int i) { return win::tile_at(tl, t_begin + warp + i * kNW); };
-  // block of this lane's key (lane & 15) of tile i; -1 when the key is not visible
+  auto seen = [&](int key) { return key < L && (key >= lo || key < a.sinks); };
+  // block id of tile i (one_block), or of this lane's key (lane & 15) of it, as the table
+  // has it: it is looked at a pass later, when it has arrived
   auto block_of = [&](int i) -> int32_t {
     if (i >= ntiles) return -1;
-    const int key = key_tile(i) * kKeys + (lane & 15);
-    if (!(key < L && (key >= lo || key < a.sinks))) return -1;
-    const int32_t b = __ldg(bt + key / a.bs);
-    if (b < 0 || b >= a.num_blocks) {
-      bad = true;
-      return -1;
-    }
-    return b;
+    const int key0 = key_tile(i) * kKeys, key = key0 + (lane & 15);
+    if (!one_block && !seen(key)) return -1;
+    return __ldg(bt + a.bs.div(one_block ? key0 : key));
   };
-  int32_t blk = block_of(0);
-  uint32_t sc_prev = 0;  // exponent byte of the tile copied last ...
-  unsigned char *sc_at = nullptr;  // ... and where it goes once it has arrived
-  auto put_scale = [&]() {
+  // block ids of the next pass to be copied, asked for a pass ahead; exponent bytes of the
+  // pass copied last, stored when the next is copied (nothing waits for either)
+  int32_t blk[KT];
+  uint32_t sc[KT];
+  unsigned char *sc_at = nullptr;
+#pragma unroll
+  for (int u = 0; u < KT; ++u) {
+    blk[u] = block_of(u);
+    sc[u] = va::kQ8ExpBias;
+  }
+  auto copy_tile = [&](int i, unsigned char *st, int32_t blk, uint32_t &sc_prev) {
+    const int key0 = i < ntiles ? key_tile(i) * kKeys : 0;
+    const bool in = blk >= 0 && blk < a.num_blocks;
+    if (one_block && in && key0 + kKeys <= L &&
+        (key0 >= lo || key0 + kKeys <= a.sinks)) {
+      // every key is seen and the rows are evenly spaced
+      const int off = a.bs.mod(key0);
+      const int64_t base = blk * a.s_block * S::ES + off * tok;
+#pragma unroll
+      for (int i = 0; i < S::P / 2; ++i) {
+        const int r = (lane + 32 * i) / S::P, c = (lane + 32 * i) % S::P * 16;
+        const int64_t src = base + r * tok + c;
+        win::cp_async<16>(va::smem_addr(st + ((r * S::RB + c) ^ S::k_swz(r))), k_head + src);
+        win::cp_async<16>(va::smem_addr(st + S::oV + ((r * S::RB + c) ^ S::v_swz(r))),
+                          v_head + src);
+      }
+      if constexpr (Q8)
+        sc_prev = s_lane[blk * a.c_block + (off + (lane & 15)) * a.c_token];
+    } else {
+      const int key = key0 + (lane & 15), off = a.bs.mod(key);
+      const bool want = i < ntiles && seen(key), on = want && in;
+      bad = bad || (want && !in);
+      const int64_t row = on ? blk * a.s_block * S::ES + off * tok : 0;
+#pragma unroll
+      for (int i = 0; i < S::P / 2; ++i) {
+        const int r = (lane + 32 * i) / S::P, c = (lane + 32 * i) % S::P * 16;
+        const int64_t src = __shfl_sync(0xffffffffu, row, r) + c;
+        const bool ro = __shfl_sync(0xffffffffu, (int)on, r);
+        win::cp_async_zfill<16>(va::smem_addr(st + ((r * S::RB + c) ^ S::k_swz(r))),
+                                ro ? k_head + src : a.kc, ro);
+        win::cp_async_zfill<16>(va::smem_addr(st + S::oV + ((r * S::RB + c) ^ S::v_swz(r))),
+                                ro ? v_head + src : a.vc, ro);
+      }
+      if constexpr (Q8)
+        sc_prev = on ? s_lane[blk * a.c_block + off * a.c_token] : va::kQ8ExpBias;
+    }
+  };
+  int wslot = 0;  // ring slot of the next pass
+  auto copy_pass = [&](int p) {
     if constexpr (Q8) {
       if (sc_at) {
-        if (lane < 16)  // K: fp32 2^e; V: fp16 2^e
-          reinterpret_cast<uint32_t *>(sc_at)[lane] = sc_prev << 23;
-        else
-          reinterpret_cast<uint16_t *>(sc_at)[lane + 16] = (uint16_t)va::q8_scale_h2(sc_prev);
+#pragma unroll
+        for (int u = 0; u < KT; ++u) {
+          unsigned char *at = sc_at + u * S::kStage;
+          if (lane < 16)  // K: fp32 2^e; V: fp16 2^e
+            reinterpret_cast<uint32_t *>(at)[lane] = sc[u] << 23;
+          else
+            reinterpret_cast<uint16_t *>(at)[lane + 16] = (uint16_t)va::q8_scale_h2(sc[u]);
+        }
       }
+      sc_at = nullptr;
     }
-  };
-  auto copy_tile = [&](int i) {
-    put_scale();
-    sc_at = nullptr;
-    if (i < ntiles) {
-      unsigned char *st = ring + (i % S::kStages) * S::kStage;
-      const int key0 = key_tile(i) * kKeys;
-      const int off = one_block ? key0 % a.bs + (lane & 15) : (key0 + (lane & 15)) % a.bs;
-      const bool on = blk >= 0;
-      const int64_t row = on ? blk * a.s_block + head_off + off * a.s_token : 0;
+    if (p < npass) {
+      unsigned char *st = ring + wslot * S::kStage;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {  // K rows g, g + 8
-        const int64_t rr = __shfl_sync(0xffffffffu, row, g + 8 * r);
-        const bool ro = __shfl_sync(0xffffffffu, (int)on, g + 8 * r);
+      for (int u = 0; u < KT; ++u) copy_tile(p * KT + u, st + u * S::kStage, blk[u], sc[u]);
+      if constexpr (Q8) sc_at = st + S::oS;
 #pragma unroll
-        for (int c = 0; c < S::KN; ++c)
-          win::cp_async_zfill<S::KB>(
-              va::smem_addr(st + ((r * S::KN + c) * 32 + lane) * S::KB),
-              a.kc + (rr + c * 4 * S::KE + t * S::KE) * S::ES, ro);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {  // V rows 2t, 2t + 1, 2t + 8, 2t + 9
-        const int k = 2 * t + (r & 1) + 8 * (r >> 1);
-        const int64_t rr = __shfl_sync(0xffffffffu, row, k);
-        const bool ro = __shfl_sync(0xffffffffu, (int)on, k);
-#pragma unroll
-        for (int c = 0; c < S::VN; ++c)
-          win::cp_async_zfill<S::VB>(
-              va::smem_addr(st + S::oV + ((r * S::VN + c) * 32 + lane) * S::VB),
-              a.vc + (rr + c * 8 * S::VE + g * S::VE) * S::ES, ro);
-      }
-      if constexpr (Q8) {  // lanes 0..15: the K exponents, 16..31: V's
-        const uint8_t *p = (lane < 16 ? a.ks : a.vs) + (on ? blk * a.c_block + c_head_off +
-                                                                 off * a.c_token
-                                                           : 0);
-        sc_prev = on ? *p : va::kQ8ExpBias;
-        sc_at = st + S::oS;
-      }
-      blk = block_of(i + 1);
+      for (int u = 0; u < KT; ++u) blk[u] = block_of((p + 1) * KT + u);
+      wslot = wslot + KT == R ? 0 : wslot + KT;
     }
     win::cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < S::kStages - 1; ++i) copy_tile(i);
+  for (int p = 0; p < R / KT - 1; ++p) copy_pass(p);
 
   float m[NT][2], l[NT][2], o[NT][D / 16][4];
 #pragma unroll
@@ -266,64 +299,77 @@ __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
     for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
   }
 
+  int rslot = 0;
 #pragma unroll 1
-  for (int i = 0; i < ntiles; ++i) {
-    copy_tile(i + S::kStages - 1);
-    win::cp_async_wait<S::kStages - 1>();
-    __syncwarp();  // the scales were stored by other lanes
-    const unsigned char *st = ring + (i % S::kStages) * S::kStage;
-    const int key0 = key_tile(i) * kKeys;
+  for (int i = 0; i < npass; ++i) {
+    copy_pass(i + R / KT - 1);
+    win::cp_async_wait<R / KT - 1>();
+    __syncwarp();  // other lanes' copies and exponents
+    const unsigned char *st0 = ring + rslot * S::kStage;
     // ---- S^T = K Q^T ----
-    float s[NT][4];
+    float s[KT][NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int u = 0; u < KT; ++u) {
+      const unsigned char *st = st0 + u * S::kStage;
 #pragma unroll
-    for (int c = 0; c < S::KN; ++c) {
-      uint32_t wa[S::KB / 4], wb[S::KB / 4];
-      lds<S::KB>(wa, st + (c * 32 + lane) * S::KB);
-      lds<S::KB>(wb, st + ((S::KN + c) * 32 + lane) * S::KB);
+      for (int n = 0; n < NT; ++n) s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = 0.f;
 #pragma unroll
-      for (int x = 0; x < S::KE / 4; ++x) {
-        uint32_t a0, a1, a2, a3;
-        if constexpr (Q8) {
-          a0 = va::q8_decode2(wa[x]);
-          a2 = va::q8_decode2(wa[x] >> 16);
-          a1 = va::q8_decode2(wb[x]);
-          a3 = va::q8_decode2(wb[x] >> 16);
-        } else {
-          a0 = wa[2 * x];
-          a2 = wa[2 * x + 1];
-          a1 = wb[2 * x];
-          a3 = wb[2 * x + 1];
+      for (int c = 0; c < S::KN; ++c) {
+        uint32_t wa[S::KB / 4], wb[S::KB / 4];
+        const int at = (g * S::RB + c * 4 * S::KB + t * S::KB) ^ S::k_swz(g);
+        lds<S::KB>(wa, st + at);
+        lds<S::KB>(wb, st + at + 8 * S::RB);  // row g + 8 is exchanged like row g
+#pragma unroll
+        for (int x = 0; x < S::KE / 4; ++x) {
+          uint32_t a0, a1, a2, a3;
+          if constexpr (Q8) {
+            a0 = va::q8_decode2(wa[x]);
+            a2 = va::q8_decode2(wa[x] >> 16);
+            a1 = va::q8_decode2(wb[x]);
+            a3 = va::q8_decode2(wb[x] >> 16);
+          } else {
+            a0 = wa[2 * x];
+            a2 = wa[2 * x + 1];
+            a1 = wb[2 * x];
+            a3 = wb[2 * x + 1];
+          }
+          const int ks = c * (S::KE / 4) + x;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma(s[u][n], a0, a1, a2, a3, qf[n][ks][0], qf[n][ks][1]);
         }
-        const int ks = c * (S::KE / 4) + x;
+      }
+      // ---- scale, mask (rows g, g + 8 of the tile; columns 2t, 2t + 1) ----
+      float fa = a.scale_log2, fb = a.scale_log2;
+      if constexpr (Q8) {
+        const float *f = reinterpret_cast<const float *>(st + S::oS);
+        fa *= f[g];
+        fb *= f[g + 8];
+      }
+      const int key0 = i * KT + u < ntiles ? key_tile(i * KT + u) * kKeys : L;
+      const bool sa = seen(key0 + g), sb = seen(key0 + g + 8);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) mma(s[n], a0, a1, a2, a3, qf[n][ks][0], qf[n][ks][1]);
+      for (int n = 0; n < NT; ++n) {
+        s[u][n][0] = sa ? s[u][n][0] * fa : -INFINITY;
+        s[u][n][1] = sa ? s[u][n][1] * fa : -INFINITY;
+        s[u][n][2] = sb ? s[u][n][2] * fb : -INFINITY;
+        s[u][n][3] = sb ? s[u][n][3] * fb : -INFINITY;
       }
     }
-    // ---- scale, mask, online softmax (rows g, g + 8 of the tile; columns 2t, 2t + 1) ----
-    float fa = a.scale_log2, fb = a.scale_log2;
-    if constexpr (Q8) {
-      const float *f = reinterpret_cast<const float *>(st + S::oS);
-      fa *= f[g];
-      fb *= f[g + 8];
-    }
-    const int ka = key0 + g, kb = ka + 8;
-    const bool va_ = ka < L && (ka >= lo || ka < a.sinks);
-    const bool vb_ = kb < L && (kb >= lo || kb < a.sinks);
-    uint32_t pb[NT][2];
+    // ---- online softmax ----
+    uint32_t pb[KT][NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float x0 = va_ ? s[n][0] * fa : -INFINITY, x1 = va_ ? s[n][1] * fa : -INFINITY;
-      float y0 = vb_ ? s[n][2] * fb : -INFINITY, y1 = vb_ ? s[n][3] * fb : -INFINITY;
-      float m0 = fmaxf(x0, y0), m1 = fmaxf(x1, y1);
+      float m0 = m[n][0], m1 = m[n][1];
+#pragma unroll
+      for (int u = 0; u < KT; ++u) {
+        m0 = fmaxf(m0, fmaxf(s[u][n][0], s[u][n][2]));
+        m1 = fmaxf(m1, fmaxf(s[u][n][1], s[u][n][3]));
+      }
 #pragma unroll
       for (int w = 4; w < 32; w <<= 1) {
         m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, w));
         m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, w));
       }
-      m0 = fmaxf(m0, m[n][0]);
-      m1 = fmaxf(m1, m[n][1]);
       if (__any_sync(0xffffffffu, m0 != m[n][0] || m1 != m[n][1])) {
         const float f0 = m0 == m[n][0] ? 1.f : va::fast_exp2(m[n][0] - m0);
         const float f1 = m1 == m[n][1] ? 1.f : va::fast_exp2(m[n][1] - m1);
@@ -339,52 +385,61 @@ __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
           o[n][k][3] *= f1;
         }
       }
-      // every tile holds a visible key, so m is finite unless a score is not
-      x0 = va::fast_exp2(x0 - m0);
-      x1 = va::fast_exp2(x1 - m1);
-      y0 = va::fast_exp2(y0 - m0);
-      y1 = va::fast_exp2(y1 - m1);
-      l[n][0] += x0 + y0;
-      l[n][1] += x1 + y1;
-      pb[n][0] = transpose8x8(va::pack_h2(x0, x1));
-      pb[n][1] = transpose8x8(va::pack_h2(y0, y1));
-    }
-    // ---- O^T += V^T P^T ----
-    uint32_t f01 = 0, f89 = 0;
-    if constexpr (Q8) {
-      const uint32_t *f = reinterpret_cast<const uint32_t *>(st + S::oS + 64);
-      f01 = f[t];
-      f89 = f[t + 4];
-    }
+      // every pass holds a visible key, so m is finite unless a score is not
 #pragma unroll
-    for (int c = 0; c < S::VN; ++c) {
-      uint32_t w[4][S::VB / 4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        lds<S::VB>(w[r], st + S::oV + ((r * S::VN + c) * 32 + lane) * S::VB);
-#pragma unroll
-      for (int x = 0; x < S::VE / 2; ++x) {  // values 2x, 2x + 1 of the copy
-        uint32_t a0, a1, a2, a3;
-        if constexpr (Q8) {
-          const uint32_t sel = x & 1 ? 0x7362 : 0x5140;
-          const uint32_t u = __byte_perm(w[0][x / 2], w[1][x / 2], sel);
-          const uint32_t v = __byte_perm(w[2][x / 2], w[3][x / 2], sel);
-          a0 = va::hmul2(va::q8_decode2(u), f01);
-          a1 = va::hmul2(va::q8_decode2(u >> 16), f01);
-          a2 = va::hmul2(va::q8_decode2(v), f89);
-          a3 = va::hmul2(va::q8_decode2(v >> 16), f89);
-        } else {
-          a0 = __byte_perm(w[0][x], w[1][x], 0x5410);
-          a1 = __byte_perm(w[0][x], w[1][x], 0x7632);
-          a2 = __byte_perm(w[2][x], w[3][x], 0x5410);
-          a3 = __byte_perm(w[2][x], w[3][x], 0x7632);
-        }
-        const int k = c * (S::VE / 2) + x;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) mma(o[n][k], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+      for (int u = 0; u < KT; ++u) {
+        const float x0 = va::fast_exp2(s[u][n][0] - m0), x1 = va::fast_exp2(s[u][n][1] - m1);
+        const float y0 = va::fast_exp2(s[u][n][2] - m0), y1 = va::fast_exp2(s[u][n][3] - m1);
+        l[n][0] += x0 + y0;
+        l[n][1] += x1 + y1;
+        pb[u][n][0] = transpose8x8(va::pack_h2(x0, x1));
+        pb[u][n][1] = transpose8x8(va::pack_h2(y0, y1));
       }
     }
-    __syncwarp();  // the next copy stores scales over this stage's
+    // ---- O^T += V^T P^T ----
+#pragma unroll
+    for (int u = 0; u < KT; ++u) {
+      const unsigned char *st = st0 + u * S::kStage;
+      uint32_t f01 = 0, f89 = 0;
+      if constexpr (Q8) {
+        const uint32_t *f = reinterpret_cast<const uint32_t *>(st + S::oS + 64);
+        f01 = f[t];
+        f89 = f[t + 4];
+      }
+#pragma unroll
+      for (int c = 0; c < S::VN; ++c) {
+        uint32_t w[4][S::VB / 4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          // rows 2t, 2t + 1, 2t + 8, 2t + 9 are exchanged alike
+          lds<S::VB>(w[r], st + S::oV + (((2 * t + (r & 1)) * S::RB + c * 8 * S::VB + g * S::VB) ^
+                                         S::v_swz(2 * t)) +
+                               (r >> 1) * 8 * S::RB);
+#pragma unroll
+        for (int x = 0; x < S::VE / 2; ++x) {  // values 2x, 2x + 1 of the copy
+          uint32_t a0, a1, a2, a3;
+          if constexpr (Q8) {
+            const uint32_t sel = x & 1 ? 0x7362 : 0x5140;
+            const uint32_t p = __byte_perm(w[0][x / 2], w[1][x / 2], sel);
+            const uint32_t q = __byte_perm(w[2][x / 2], w[3][x / 2], sel);
+            a0 = va::hmul2(va::q8_decode2(p), f01);
+            a1 = va::hmul2(va::q8_decode2(p >> 16), f01);
+            a2 = va::hmul2(va::q8_decode2(q), f89);
+            a3 = va::hmul2(va::q8_decode2(q >> 16), f89);
+          } else {
+            a0 = __byte_perm(w[0][x], w[1][x], 0x5410);
+            a1 = __byte_perm(w[0][x], w[1][x], 0x7632);
+            a2 = __byte_perm(w[2][x], w[3][x], 0x5410);
+            a3 = __byte_perm(w[2][x], w[3][x], 0x7632);
+          }
+          const int k = c * (S::VE / 2) + x;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma(o[n][k], a0, a1, a2, a3, pb[u][n][0], pb[u][n][1]);
+        }
+      }
+    }
+    rslot = rslot + KT == R ? 0 : rslot + KT;
+    __syncwarp();  // the next copies go over this pass's slots
   }
   win::cp_async_wait<0>();
 #pragma unroll
@@ -397,18 +452,18 @@ __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
   if (bad) s_bad = 1;
   __syncthreads();  // the ring is free: the warps' results go there
 
-  constexpr int NH = 8 * NT;
-  float *so = reinterpret_cast<float *>(smem);     // [kNW][NH][D]
-  float *sm = so + kNW * NH * D, *sl = sm + kNW * NH;  // [kNW][NH]
+  // value e of lane g lies at e * 8 + g of its head's row: stores hit every bank once
+  constexpr int NH = 8 * NT, HS = S::kHead;
+  float *so = reinterpret_cast<float *>(smem);          // [kNW][NH][HS]
+  float *sm = so + kNW * NH * HS, *sl = sm + kNW * NH;  // [kNW][NH]
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int k = 0; k < D / 16; ++k)
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const int e = 2 * k + y, d = e / S::VE * (8 * S::VE) + g * S::VE + e % S::VE;
-        so[(warp * NH + n * 8 + 2 * t) * D + d] = o[n][k][2 * y];
-        so[(warp * NH + n * 8 + 2 * t + 1) * D + d] = o[n][k][2 * y + 1];
+        so[(warp * NH + n * 8 + 2 * t) * HS + (2 * k + y) * 8 + g] = o[n][k][2 * y];
+        so[(warp * NH + n * 8 + 2 * t + 1) * HS + (2 * k + y) * 8 + g] = o[n][k][2 * y + 1];
       }
     if (g == 0) {
 #pragma unroll
@@ -423,6 +478,7 @@ __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
   if (skip && threadIdx.x == 0) va::raise_flag(a.err, VA_FLAG_BAD_BLOCK);
   for (int i = threadIdx.x; i < nheads * D; i += kNW * 32) {
     const int h = i / D, d = i - h * D;
+    const int at = (d / (8 * S::VE) * S::VE + d % S::VE) * 8 + d / S::VE % 8;
     float M = sm[h];
 #pragma unroll
     for (int w = 1; w < kNW; ++w) M = fmaxf(M, sm[w * NH + h]);
@@ -431,7 +487,7 @@ __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
     for (int w = 0; w < kNW; ++w) {
       // a warp without tiles has m = -inf and adds nothing
       const float f = sm[w * NH + h] == -INFINITY ? 0.f : va::fast_exp2(sm[w * NH + h] - M);
-      A += so[(w * NH + h) * D + d] * f;
+      A += so[(w * NH + h) * HS + at] * f;
       Ls += sl[w * NH + h] * f;
     }
     if (nsplit == 1) {
@@ -446,36 +502,55 @@ __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
   }
 }
 
-// Merges the ranges of the sequences that have more than one, in range order; one thread
-// per output value.
-__global__ void __launch_bounds__(256) window_decode_merge_kernel(const Args a, int D) {
+// Merges the ranges of a sequence that has more than one, in an order that only its length
+// sets: a CTA per (sequence, query head), warp w takes ranges w, w + 4, ..., each lane
+// D / 32 of the values, then the warps' sums are added in warp order.
+template <int D>
+__global__ void __launch_bounds__(128) window_decode_merge_kernel(const Args a) {
+  constexpr int E = D / 32;
+  __shared__ float s_acc[4][D], s_l[4];
   va::pdl_enter();
-  const int seq = blockIdx.x;
+  const int seq = blockIdx.x, h = blockIdx.y;
   const int L = seq_len(a, seq, false);
   if (L == 0) return;
   const win::Tiles tl = win::key_tiles(L - 1, L - 1, a.window, a.sinks, kKeys);
   const int nsplit = (tl.count + a.tps - 1) / a.tps;
   if (nsplit == 1) return;
-  const int i = blockIdx.y * 256 + threadIdx.x;
-  if (i >= a.Hq * D) return;
-  const int h = i / D, d = i - h * D;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t p = ((int64_t)seq * a.Hq + h) * a.splits;
-  float M = -INFINITY, A = 0.f, Ls = 0.f;
+  // every warp finds the common maximum, 32 ranges at a time
+  float M = -INFINITY;
   bool skip = false;
-  for (int s = 0; s < nsplit; ++s) {
+  for (int s = lane; s < nsplit; s += 32) {
     const float2 v = a.ws_ml[p + s];
     skip = skip || v.y < 0.f;
     M = fmaxf(M, v.x);
   }
-  if (skip) return;
-#pragma unroll 4
-  for (int s = 0; s < nsplit; ++s) {
+  if (__any_sync(0xffffffffu, skip)) return;  // uniform: every warp sees every range
+#pragma unroll
+  for (int w = 1; w < 32; w <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, w));
+  float A[E], Ls = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) A[e] = 0.f;
+#pragma unroll 8
+  for (int s = warp; s < nsplit; s += 4) {
     const float2 v = a.ws_ml[p + s];
     const float f = v.x == -INFINITY ? 0.f : va::fast_exp2(v.x - M);
-    A = fmaf(a.ws_acc[(p + s) * D + d], f, A);
     Ls = fmaf(v.y, f, Ls);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      A[e] = fmaf(a.ws_acc[(p + s) * D + e * 32 + lane], f, A[e]);
   }
-  a.out[seq * a.o_s_token + (int64_t)h * a.o_s_head + d] = __float2half_rn(A / Ls);
+#pragma unroll
+  for (int e = 0; e < E; ++e) s_acc[warp][e * 32 + lane] = A[e];
+  if (lane == 0) s_l[warp] = Ls;
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d < D) {
+    const float acc = (s_acc[0][d] + s_acc[1][d]) + (s_acc[2][d] + s_acc[3][d]);
+    const float sum = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    a.out[seq * a.o_s_token + (int64_t)h * a.o_s_head + d] = __float2half_rn(acc / sum);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -489,7 +564,7 @@ struct Plan {
 // Head groups of up to 16; ranges so that about kTargetCtas CTAs have work, at least two
 // tiles per warp each.
 Plan make_plan(int64_t num_seqs, int Hq, int Hkv, int D, int64_t max_len, int window, int sinks) {
-  constexpr int64_t kTargetCtas = 148 * 6;
+  constexpr int64_t kTargetCtas = 148 * 24;
   Plan p{};
   const int G = Hq / Hkv;
   p.hg = (G + 15) / 16;
@@ -516,15 +591,14 @@ Plan make_plan(int64_t num_seqs, int Hq, int Hkv, int D, int64_t max_len, int wi
 
 template <int D, bool Q8, int NT>
 int launch_t(const Args &a, dim3 grid, cudaStream_t st) {
-  constexpr int merge = kNW * 8 * NT * (D + 2) * 4;
+  constexpr int merge = kNW * 8 * NT * (Shape<D, Q8>::kHead + 2) * 4;
   constexpr int smem = Shape<D, Q8>::kRing > merge ? Shape<D, Q8>::kRing : merge;
   static std::atomic<uint64_t> done{0};
   if (!win::allow_smem(window_decode_kernel<D, Q8, NT>, smem, done)) return VA_ERR_LAUNCH;
   if (va_host::launch_pdl_smem(window_decode_kernel<D, Q8, NT>, grid, kNW * 32, smem, st, a))
     return VA_ERR_LAUNCH;
   if (a.splits > 1 &&
-      va_host::launch_pdl(window_decode_merge_kernel,
-                          dim3(grid.z, (unsigned)((a.Hq * D + 255) / 256)), 256, st, a, D))
+      va_host::launch_pdl(window_decode_merge_kernel<D>, dim3(grid.z, (unsigned)a.Hq), 128, st, a))
     return VA_ERR_LAUNCH;
   return va_host::launch_status();
 }
@@ -582,7 +656,7 @@ extern "C" int va_window_decode(void *out, const void *q, void *k_cache, void *v
     return VA_ERR_INVALID_ARG;
   const Plan p = make_plan(num_seqs, num_query_heads, num_kv_heads, head_size, max_seq_len,
                            window, sink_tokens);
-  if ((int64_t)num_kv_heads * p.hg > 65535) return VA_ERR_UNSUPPORTED;
+  if (num_query_heads > 65535) return VA_ERR_UNSUPPORTED;
   if (p.total && (!workspace || workspace_bytes < p.total || !va_host::aligned16(workspace)))
     return VA_ERR_WORKSPACE;
   Args a{};
@@ -607,7 +681,7 @@ extern "C" int va_window_decode(void *out, const void *q, void *k_cache, void *v
   a.G = num_query_heads / num_kv_heads;
   a.hg = p.hg;
   a.gc = p.gc;
-  a.bs = block_size;
+  a.bs = win::fast_div(block_size);
   a.window = win::window_of(window);
   a.sinks = sink_tokens;
   a.tps = p.tps;
