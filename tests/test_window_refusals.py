@@ -44,12 +44,13 @@ def test_window_decode_workspace(lib):
     f = lib.va_window_decode_workspace_size
     assert f(0, 32, 8, 128, 4096, 0, 0) == 0
     assert f(4, 32, 5, 128, 4096, 0, 0) == 0
-    assert f(1024, 32, 8, 128, 8192, 0, 0) == 0      # enough sequences: none is cut
+    assert f(4096, 32, 8, 128, 8192, 0, 0) == 0      # enough sequences: none is cut
     assert f(1, 32, 8, 128, 64, 0, 0) == 0           # too short to cut
     big = f(1, 32, 8, 128, 131072, 0, 0)
     assert big > 0 and big % 256 == 0
     # a short window bounds what there is to cut, however long the sequences
-    assert f(1, 32, 8, 128, 1 << 30, 64, 4) < big
+    assert f(1, 32, 8, 128, 1 << 30, 64, 4) == 0
+    assert 0 < f(1, 32, 8, 128, 1 << 30, 1000, 4) < big
 
 
 def _write(lib, D=128, T=4, H=8, bs=16, nb=64, ptr=16, st=(16384, 2048, 128), new=(1024, 128)):

@@ -21,9 +21,11 @@
 //   * Statistics, sums and O are fp32; P is rounded to fp16 (2^-11 of a value <= 1) for
 //     the second product.  An e4m3 code becomes fp16 exactly; the exponent of a K row
 //     scales its fp32 score, that of a V row its fp16 values (both exact).
-//   * Long contexts with few sequences are cut into ranges of tiles, one CTA each; the
-//     ranges' (O, m, l) are merged in range order by a second kernel launched as a
-//     programmatic dependent.
+//   * All tiles of the call, in (sequence, head group, tile) order, are one list that is cut
+//     into equal ranges, one per CTA that fits the GPU: ragged lengths, one long sequence or
+//     many short ones all make one even wave.  A range holds whole (sequence, head group)
+//     lists, written at once, and at most two parts of lists, whose (O, m, l) a second
+//     kernel, launched as a programmatic dependent, merges in list order.
 //   * Keys that the query does not see are zero-filled, never read: what lies in the
 //     cache behind a sequence, before its window or in a freed block does not matter.
 #include "window.cuh"
@@ -68,11 +70,12 @@ struct Args {
   uint8_t *ks, *vs;   // exponent bytes (e4m3 caches)
   const __half *nk, *nv;
   const int32_t *bt, *sl;
-  float *ws_acc;
-  float2 *ws_ml;
+  float *ws_acc;     // [2 * ranges][gc][D] un-normalised O of the ranges' first and last parts
+  float2 *ws_ml;     // [2 * ranges][gc] (m, l) of them; l < 0: a block could not be read
+  int64_t *ws_plan;  // {tiles per range, tiles before sequence 0, 1, ...}
   int32_t *err;
   int64_t max_blocks, num_blocks, max_len;
-  int Hq, G, hg, gc, window, sinks, tps, splits;
+  int B, Hq, G, hg, gc, Hk, window, sinks, ranges;
   win::FastDiv bs;
   float scale_log2;
   int64_t s_block, s_head, s_token, c_block, c_head, c_token;
@@ -115,6 +118,69 @@ VA_DEVINL int seq_len(const Args &a, int seq, bool flag) {
   }
   return L;
 }
+VA_DEVINL win::Tiles seq_tiles(const Args &a, int L) {
+  return win::key_tiles(L - 1, L - 1, a.window, a.sinks, kKeys);
+}
+VA_DEVINL int num_tiles(const Args &a, int L) { return L > 0 ? seq_tiles(a, L).count : 0; }
+
+// Fewest tiles of a range: two per warp.
+constexpr int kMinRange = 2 * kNW;
+
+// The range of this CTA in the list of all tiles in (sequence, head group, tile) order.
+struct Range {
+  int64_t begin, end;  // tiles of the list
+  int64_t before;      // tiles of one head group before sequence `seq`
+  int seq;             // sequence of the first tile
+};
+// Every CTA sums the sequences' tiles for itself (their lengths are few and in L2), so no
+// planning kernel runs before; CTA 0 leaves the sums for the merge.
+VA_DEVINL Range find_range(const Args &a) {
+  __shared__ int64_t s_warp[kNW];
+  __shared__ int64_t s_before;
+  __shared__ int s_seq;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (a.B + kNW * 32 - 1) / (kNW * 32);
+  const int q0 = min(tid * per, a.B), q1 = min(q0 + per, a.B);
+  int64_t mine = 0;
+  for (int q = q0; q < q1; ++q) mine += num_tiles(a, seq_len(a, q, blockIdx.x == 0));
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += x;
+  }
+  if (lane == 31) s_warp[warp] = incl;
+  __syncthreads();
+  int64_t total = 0, at = incl - mine;
+#pragma unroll
+  for (int w = 0; w < kNW; ++w) {
+    if (w < warp) at += s_warp[w];
+    total += s_warp[w];
+  }
+  total *= a.Hk;
+  const int64_t w = max((total + a.ranges - 1) / a.ranges, (int64_t)kMinRange);
+  Range r;
+  r.begin = blockIdx.x * w;
+  r.end = min(r.begin + w, total);
+  if (r.begin >= at * a.Hk && r.begin < (at + mine) * a.Hk) {  // one thread's sequences hold it
+    int q = q0;
+    int64_t x = at;
+    for (int n; x + (n = num_tiles(a, seq_len(a, q, false))) <= r.begin / a.Hk; ++q) x += n;
+    s_before = x;
+    s_seq = q;
+  }
+  if (blockIdx.x == 0) {
+    if (tid == 0) a.ws_plan[0] = w;
+    for (int q = q0; q < q1; ++q) {
+      a.ws_plan[1 + q] = at;
+      at += num_tiles(a, seq_len(a, q, false));
+    }
+  }
+  __syncthreads();
+  r.before = s_before;  // not set, and not used, where the range is empty
+  r.seq = s_seq;
+  return r;
+}
 
 // The new K (threads 0..15) and V (threads 16..31) row of one kv head into the cache.
 template <int D, bool Q8>
@@ -148,28 +214,20 @@ VA_DEVINL void write_new_row(const Args &a, int seq, int kvh, int64_t blk, int o
   }
 }
 
-// NT: tiles of 8 query heads per warp (1 for groups of up to 8, 2 up to 16).
+// One part: tiles [t_begin, t_end) of one head group of one sequence.  `slot` >= 0: not
+// the whole list of its tiles, so the result goes to that slot of the workspace.
 template <int D, bool Q8, int NT>
-__global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
+VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int &s_bad, int seq, int hk, int L,
+                           const win::Tiles &tl, int t_begin, int t_end, int64_t slot) {
   using S = Shape<D, Q8>;
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int s_bad;
-  va::pdl_enter();
-  const int split = blockIdx.x, seq = blockIdx.z;
-  const int kvh = blockIdx.y / a.hg, head0 = kvh * a.G + (blockIdx.y - kvh * a.hg) * a.gc;
+  const int kvh = hk / a.hg, head0 = kvh * a.G + (hk - kvh * a.hg) * a.gc;
   const int nheads = min(a.gc, (kvh + 1) * a.G - head0);
-  const int L = seq_len(a, seq, split == 0 && blockIdx.y == 0 && threadIdx.x == 0);
-  if (L == 0) return;
-  const win::Tiles tl = win::key_tiles(L - 1, L - 1, a.window, a.sinks, kKeys);
-  const int t_begin = split * a.tps, t_end = min(t_begin + a.tps, tl.count);
-  if (t_begin >= t_end) return;
-  const int nsplit = (tl.count + a.tps - 1) / a.tps;
   const int lo = win::run_start(L - 1, a.window);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int32_t *bt = a.bt + seq * a.max_blocks;
   if (threadIdx.x == 0) s_bad = 0;
 
-  // The CTA that reads the newest key writes it first, then reads it back with the rest.
+  // The part that reads the newest key writes it first, then reads it back with the rest.
   if (a.nk && t_end == tl.count) {
     const int page = a.bs.div(L - 1);
     const int32_t blk = __ldg(bt + page);
@@ -490,39 +548,81 @@ __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
       A += so[(w * NH + h) * HS + at] * f;
       Ls += sl[w * NH + h] * f;
     }
-    if (nsplit == 1) {
+    if (slot < 0) {
       if (!skip)
         a.out[seq * a.o_s_token + (int64_t)(head0 + h) * a.o_s_head + d] = __float2half_rn(A / Ls);
     } else {
-      const int64_t p = ((int64_t)seq * a.Hq + head0 + h) * a.splits + split;
+      const int64_t p = slot * a.gc + h;
       a.ws_acc[p * D + d] = A;
-      // l < 0 marks a range with an unreadable block: its sequence is left alone
+      // l < 0 marks a part with an unreadable block: its sequence is left alone
       if (d == 0) a.ws_ml[p] = make_float2(M, skip ? -1.f : Ls);
     }
   }
 }
 
-// Merges the ranges of a sequence that has more than one, in an order that only its length
-// sets: a CTA per (sequence, query head), warp w takes ranges w, w + 4, ..., each lane
-// D / 32 of the values, then the warps' sums are added in warp order.
+// NT: tiles of 8 query heads per warp (1 for groups of up to 8, 2 up to 16).
+template <int D, bool Q8, int NT>
+__global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int s_bad;
+  va::pdl_enter();
+  if (a.ranges == 0) {  // a CTA per (sequence, head group)
+    const int seq = blockIdx.x / a.Hk, hk = blockIdx.x - seq * a.Hk;
+    const int L = seq_len(a, seq, hk == 0 && threadIdx.x == 0);
+    if (L == 0) return;
+    const win::Tiles tl = seq_tiles(a, L);
+    decode_part<D, Q8, NT>(a, smem, s_bad, seq, hk, L, tl, 0, tl.count, -1);
+    return;
+  }
+  const Range r = find_range(a);
+  int seq = r.seq;
+  int64_t before = r.before;
+#pragma unroll 1
+  for (int64_t at = r.begin; at < r.end;) {
+    const int L = seq_len(a, seq, false), n = num_tiles(a, L);
+    const int64_t rel = at - before * a.Hk;
+    if (rel >= (int64_t)n * a.Hk) {  // past this sequence (also where it has no tiles)
+      before += n;
+      ++seq;
+      continue;
+    }
+    const int hk = (int)(rel / n), t_begin = (int)(rel - (int64_t)hk * n);
+    const int t_end = (int)min((int64_t)n, t_begin + (r.end - at));
+    const int64_t slot =
+        t_begin == 0 && t_end == n ? -1 : 2 * (int64_t)blockIdx.x + (at == r.begin ? 0 : 1);
+    decode_part<D, Q8, NT>(a, smem, s_bad, seq, hk, L, seq_tiles(a, L), t_begin, t_end, slot);
+    __syncthreads();  // the merged sums have been read
+    at += t_end - t_begin;
+  }
+}
+
+// Merges the parts of a (sequence, query head) that lies in more than one range, in an
+// order that only the lengths set: a CTA per pair, warp w takes parts w, w + 4, ..., each
+// lane D / 32 of the values, then the warps' sums are added in warp order.
 template <int D>
 __global__ void __launch_bounds__(128) window_decode_merge_kernel(const Args a) {
   constexpr int E = D / 32;
   __shared__ float s_acc[4][D], s_l[4];
   va::pdl_enter();
   const int seq = blockIdx.x, h = blockIdx.y;
-  const int L = seq_len(a, seq, false);
-  if (L == 0) return;
-  const win::Tiles tl = win::key_tiles(L - 1, L - 1, a.window, a.sinks, kKeys);
-  const int nsplit = (tl.count + a.tps - 1) / a.tps;
-  if (nsplit == 1) return;
+  const int n = num_tiles(a, seq_len(a, seq, false));
+  if (n == 0) return;
+  const int kvh = h / a.G, j = (h - kvh * a.G) / a.gc, hl = h - kvh * a.G - j * a.gc;
+  const int64_t width = a.ws_plan[0];
+  const int64_t first = a.ws_plan[1 + seq] * a.Hk + (int64_t)(kvh * a.hg + j) * n;
+  const int64_t c0 = first / width;
+  const int nsplit = (int)((first + n - 1) / width - c0) + 1;
+  if (nsplit == 1) return;  // written whole
+  // range c holds the pair's part in slot 0, but in slot 1 where the pair begins inside it
+  auto part = [&](int s) -> int64_t {
+    return (2 * (c0 + s) + ((c0 + s) * width < first ? 1 : 0)) * a.gc + hl;
+  };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t p = ((int64_t)seq * a.Hq + h) * a.splits;
   // every warp finds the common maximum, 32 ranges at a time
   float M = -INFINITY;
   bool skip = false;
   for (int s = lane; s < nsplit; s += 32) {
-    const float2 v = a.ws_ml[p + s];
+    const float2 v = a.ws_ml[part(s)];
     skip = skip || v.y < 0.f;
     M = fmaxf(M, v.x);
   }
@@ -534,12 +634,13 @@ __global__ void __launch_bounds__(128) window_decode_merge_kernel(const Args a) 
   for (int e = 0; e < E; ++e) A[e] = 0.f;
 #pragma unroll 8
   for (int s = warp; s < nsplit; s += 4) {
-    const float2 v = a.ws_ml[p + s];
+    const int64_t p = part(s);
+    const float2 v = a.ws_ml[p];
     const float f = v.x == -INFINITY ? 0.f : va::fast_exp2(v.x - M);
     Ls = fmaf(v.y, f, Ls);
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      A[e] = fmaf(a.ws_acc[(p + s) * D + e * 32 + lane], f, A[e]);
+      A[e] = fmaf(a.ws_acc[p * D + e * 32 + lane], f, A[e]);
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) s_acc[warp][e * 32 + lane] = A[e];
@@ -557,56 +658,72 @@ __global__ void __launch_bounds__(128) window_decode_merge_kernel(const Args a) 
 // host side
 // ---------------------------------------------------------------------------
 struct Plan {
-  int gc, hg, tps, splits;
-  size_t o_ml, total;
+  int gc, hg, most;  // most: ranges, 0 where every (sequence, head group) has its own CTA
+  size_t o_ml, o_plan, total;
 };
 
-// Head groups of up to 16; ranges so that about kTargetCtas CTAs have work, at least two
-// tiles per warp each.
+// CTAs per SM that the workspace is sized for (the kernels fit 2 to 4).
+constexpr int kMaxPerSm = 4;
+
+// Head groups of up to 16.  All tiles of the call are one list that is cut into equal
+// ranges, one per CTA that fits the GPU at once: one even wave, whatever the lengths.
+// Two cases have nothing to gain from the cut and its merge kernel: sequences of so few
+// tiles that a range is hardly shorter, and so many of them that whole ones balance.
 Plan make_plan(int64_t num_seqs, int Hq, int Hkv, int D, int64_t max_len, int window, int sinks) {
-  constexpr int64_t kTargetCtas = 148 * 24;
   Plan p{};
   const int G = Hq / Hkv;
   p.hg = (G + 15) / 16;
   p.gc = (G + p.hg - 1) / p.hg;
+  window = win::window_of(window);
   int64_t keys = max_len;
   if (window > 0 && (int64_t)window + sinks < keys) keys = (int64_t)window + sinks;
   // an unaligned run and the sinks each reach into one more tile
   const int64_t tiles = (keys + kKeys - 1) / kKeys + 2;
-  const int64_t units = num_seqs * Hkv * p.hg;
-  int64_t splits = kTargetCtas / (units > 0 ? units : 1);
-  const int64_t most = tiles / (2 * kNW);
-  if (splits > most) splits = most;
-  if (splits < 1) splits = 1;
-  const int64_t tps = (tiles + splits - 1) / splits;
-  p.tps = (int)tps;
-  p.splits = (int)((tiles + tps - 1) / tps);
-  if (p.splits > 1) {
-    const size_t parts = (size_t)num_seqs * Hq * p.splits;
-    p.o_ml = (parts * D * 4 + 255) & ~size_t(255);
-    p.total = p.o_ml + ((parts * 8 + 255) & ~size_t(255));
-  }
+  const int64_t units = num_seqs * Hkv * p.hg, slots = (int64_t)kMaxPerSm * va_host::sm_count();
+  if (tiles <= 2 * kMinRange || units >= 16 * slots) return p;
+  const int64_t most = units * ((tiles + kMinRange - 1) / kMinRange);
+  p.most = (int)(most < slots ? most : slots);
+  auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
+  p.o_ml = up((size_t)p.most * 2 * p.gc * D * 4);
+  p.o_plan = p.o_ml + up((size_t)p.most * 2 * p.gc * 8);
+  p.total = p.o_plan + up((size_t)(num_seqs + 1) * 8);
   return p;
 }
 
 template <int D, bool Q8, int NT>
-int launch_t(const Args &a, dim3 grid, cudaStream_t st) {
+int launch_t(Args &a, cudaStream_t st) {
   constexpr int merge = kNW * 8 * NT * (Shape<D, Q8>::kHead + 2) * 4;
   constexpr int smem = Shape<D, Q8>::kRing > merge ? Shape<D, Q8>::kRing : merge;
   static std::atomic<uint64_t> done{0};
+  static std::atomic<int> per_sm{0};
   if (!win::allow_smem(window_decode_kernel<D, Q8, NT>, smem, done)) return VA_ERR_LAUNCH;
-  if (va_host::launch_pdl_smem(window_decode_kernel<D, Q8, NT>, grid, kNW * 32, smem, st, a))
+  int64_t grid = (int64_t)a.B * a.Hk;
+  if (a.ranges) {
+    int n = per_sm.load(std::memory_order_relaxed);
+    if (!n) {
+      if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, window_decode_kernel<D, Q8, NT>,
+                                                        kNW * 32, smem) != cudaSuccess ||
+          n < 1)
+        return VA_ERR_LAUNCH;
+      per_sm.store(n = n < kMaxPerSm ? n : kMaxPerSm, std::memory_order_relaxed);
+    }
+    const int fit = n * va_host::sm_count();
+    if (fit < a.ranges) a.ranges = fit;
+    grid = a.ranges;
+  }
+  if (va_host::launch_pdl_smem(window_decode_kernel<D, Q8, NT>, (unsigned)grid, kNW * 32, smem, st,
+                               a))
     return VA_ERR_LAUNCH;
-  if (a.splits > 1 &&
-      va_host::launch_pdl(window_decode_merge_kernel<D>, dim3(grid.z, (unsigned)a.Hq), 128, st, a))
+  if (a.ranges && va_host::launch_pdl(window_decode_merge_kernel<D>,
+                                      dim3((unsigned)a.B, (unsigned)a.Hq), 128, st, a))
     return VA_ERR_LAUNCH;
   return va_host::launch_status();
 }
 
 template <int D>
-int launch_d(bool q8, const Args &a, dim3 grid, cudaStream_t st) {
-  if (q8) return a.gc <= 8 ? launch_t<D, true, 1>(a, grid, st) : launch_t<D, true, 2>(a, grid, st);
-  return a.gc <= 8 ? launch_t<D, false, 1>(a, grid, st) : launch_t<D, false, 2>(a, grid, st);
+int launch_d(bool q8, Args &a, cudaStream_t st) {
+  if (q8) return a.gc <= 8 ? launch_t<D, true, 1>(a, st) : launch_t<D, true, 2>(a, st);
+  return a.gc <= 8 ? launch_t<D, false, 1>(a, st) : launch_t<D, false, 2>(a, st);
 }
 
 }  // namespace
@@ -656,7 +773,8 @@ extern "C" int va_window_decode(void *out, const void *q, void *k_cache, void *v
     return VA_ERR_INVALID_ARG;
   const Plan p = make_plan(num_seqs, num_query_heads, num_kv_heads, head_size, max_seq_len,
                            window, sink_tokens);
-  if (num_query_heads > 65535) return VA_ERR_UNSUPPORTED;
+  if (num_query_heads > 65535 || num_seqs * num_kv_heads * p.hg > INT32_MAX)
+    return VA_ERR_UNSUPPORTED;
   if (p.total && (!workspace || workspace_bytes < p.total || !va_host::aligned16(workspace)))
     return VA_ERR_WORKSPACE;
   Args a{};
@@ -670,9 +788,12 @@ extern "C" int va_window_decode(void *out, const void *q, void *k_cache, void *v
   a.nv = static_cast<const __half *>(new_v);
   a.bt = block_table;
   a.sl = seq_lens;
-  a.ws_acc = static_cast<float *>(workspace);
-  a.ws_ml = p.total ? reinterpret_cast<float2 *>(static_cast<unsigned char *>(workspace) + p.o_ml)
-                    : nullptr;
+  if (p.total) {
+    unsigned char *ws = static_cast<unsigned char *>(workspace);
+    a.ws_acc = reinterpret_cast<float *>(ws);
+    a.ws_ml = reinterpret_cast<float2 *>(ws + p.o_ml);
+    a.ws_plan = reinterpret_cast<int64_t *>(ws + p.o_plan);
+  }
   a.err = err_flag;
   a.max_blocks = max_blocks_per_seq;
   a.num_blocks = num_blocks;
@@ -684,21 +805,21 @@ extern "C" int va_window_decode(void *out, const void *q, void *k_cache, void *v
   a.bs = win::fast_div(block_size);
   a.window = win::window_of(window);
   a.sinks = sink_tokens;
-  a.tps = p.tps;
-  a.splits = p.splits;
+  a.ranges = p.most;
+  a.B = (int)num_seqs;
+  a.Hk = num_kv_heads * p.hg;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.s_block = s_block; a.s_head = s_head; a.s_token = s_token;
   a.c_block = sc_block; a.c_head = sc_head; a.c_token = sc_token;
   a.q_s_token = q_s_token; a.q_s_head = q_s_head;
   a.o_s_token = o_s_token; a.o_s_head = o_s_head;
   a.n_s_token = new_s_token; a.n_s_head = new_s_head;
-  const dim3 grid((unsigned)p.splits, (unsigned)(num_kv_heads * p.hg), (unsigned)num_seqs);
   auto st = static_cast<cudaStream_t>(stream);
   switch (head_size) {
-    case 32: return launch_d<32>(kv_e4m3 != 0, a, grid, st);
-    case 64: return launch_d<64>(kv_e4m3 != 0, a, grid, st);
-    case 96: return launch_d<96>(kv_e4m3 != 0, a, grid, st);
-    case 128: return launch_d<128>(kv_e4m3 != 0, a, grid, st);
+    case 32: return launch_d<32>(kv_e4m3 != 0, a, st);
+    case 64: return launch_d<64>(kv_e4m3 != 0, a, st);
+    case 96: return launch_d<96>(kv_e4m3 != 0, a, st);
+    case 128: return launch_d<128>(kv_e4m3 != 0, a, st);
   }
   return VA_ERR_UNSUPPORTED;
 }
