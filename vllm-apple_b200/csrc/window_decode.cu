@@ -72,7 +72,7 @@ struct Args {
   const int32_t *bt, *sl;
   float *ws_acc;     // [2 * ranges][gc][D] un-normalised O of the ranges' first and last parts
   float2 *ws_ml;     // [2 * ranges][gc] (m, l) of them; l < 0: a block could not be read
-  int64_t *ws_plan;  // {tiles per range, tiles before sequence 0, 1, ...}
+  int64_t *ws_plan;  // {places per range, places before sequence 0, 1, ...}
   int32_t *err;
   int64_t max_blocks, num_blocks, max_len;
   int B, Hq, G, hg, gc, Hk, window, sinks, ranges;
@@ -126,13 +126,19 @@ VA_DEVINL int num_tiles(const Args &a, int L) { return L > 0 ? seq_tiles(a, L).c
 // Fewest tiles of a range: two per warp.
 constexpr int kMinRange = 2 * kNW;
 
-// The range of this CTA in the list of all tiles in (sequence, head group, tile) order.
+// Beginning a list of tiles (its length, block ids, first copies, the merge of the warps)
+// takes a CTA about as long as this many tiles, so every list counts for that many more
+// when the ranges are cut: its first kOpen places hold no tile.
+constexpr int kOpen = 24;
+VA_DEVINL int places(int tiles) { return tiles > 0 ? tiles + kOpen : 0; }
+
+// The range of this CTA in the list of all places in (sequence, head group, tile) order.
 struct Range {
-  int64_t begin, end;  // tiles of the list
-  int64_t before;      // tiles of one head group before sequence `seq`
-  int seq;             // sequence of the first tile
+  int64_t begin, end;  // places of the list
+  int64_t before;      // places of one head group before sequence `seq`
+  int seq;             // sequence of the first place
 };
-// Every CTA sums the sequences' tiles for itself (their lengths are few and in L2), so no
+// Every CTA sums the sequences' places for itself (their lengths are few and in L2), so no
 // planning kernel runs before; CTA 0 leaves the sums for the merge.
 VA_DEVINL Range find_range(const Args &a) {
   __shared__ int64_t s_warp[kNW];
@@ -142,7 +148,7 @@ VA_DEVINL Range find_range(const Args &a) {
   const int per = (a.B + kNW * 32 - 1) / (kNW * 32);
   const int q0 = min(tid * per, a.B), q1 = min(q0 + per, a.B);
   int64_t mine = 0;
-  for (int q = q0; q < q1; ++q) mine += num_tiles(a, seq_len(a, q, blockIdx.x == 0));
+  for (int q = q0; q < q1; ++q) mine += places(num_tiles(a, seq_len(a, q, blockIdx.x == 0)));
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -165,7 +171,7 @@ VA_DEVINL Range find_range(const Args &a) {
   if (r.begin >= at * a.Hk && r.begin < (at + mine) * a.Hk) {  // one thread's sequences hold it
     int q = q0;
     int64_t x = at;
-    for (int n; x + (n = num_tiles(a, seq_len(a, q, false))) <= r.begin / a.Hk; ++q) x += n;
+    for (int n; x + (n = places(num_tiles(a, seq_len(a, q, false)))) <= r.begin / a.Hk; ++q) x += n;
     s_before = x;
     s_seq = q;
   }
@@ -173,7 +179,7 @@ VA_DEVINL Range find_range(const Args &a) {
     if (tid == 0) a.ws_plan[0] = w;
     for (int q = q0; q < q1; ++q) {
       a.ws_plan[1 + q] = at;
-      at += num_tiles(a, seq_len(a, q, false));
+      at += places(num_tiles(a, seq_len(a, q, false)));
     }
   }
   __syncthreads();
@@ -579,20 +585,25 @@ __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
   int64_t before = r.before;
 #pragma unroll 1
   for (int64_t at = r.begin; at < r.end;) {
-    const int L = seq_len(a, seq, false), n = num_tiles(a, L);
+    const int L = seq_len(a, seq, false), n = num_tiles(a, L), np = places(n);
     const int64_t rel = at - before * a.Hk;
-    if (rel >= (int64_t)n * a.Hk) {  // past this sequence (also where it has no tiles)
-      before += n;
+    if (rel >= (int64_t)np * a.Hk) {  // past this sequence (also where it has no tiles)
+      before += np;
       ++seq;
       continue;
     }
-    const int hk = (int)(rel / n), t_begin = (int)(rel - (int64_t)hk * n);
-    const int t_end = (int)min((int64_t)n, t_begin + (r.end - at));
-    const int64_t slot =
-        t_begin == 0 && t_end == n ? -1 : 2 * (int64_t)blockIdx.x + (at == r.begin ? 0 : 1);
-    decode_part<D, Q8, NT>(a, smem, s_bad, seq, hk, L, seq_tiles(a, L), t_begin, t_end, slot);
-    __syncthreads();  // the merged sums have been read
-    at += t_end - t_begin;
+    const int hk = (int)(rel / np), p_begin = (int)(rel - (int64_t)hk * np);
+    const int p_end = (int)min((int64_t)np, p_begin + (r.end - at));
+    const int t_begin = max(p_begin - kOpen, 0), t_end = max(p_end - kOpen, 0);
+    if (t_end > t_begin) {
+      // a part of a list is the range's first (slot 0) or, where its list begins, last (1)
+      const int64_t slot = t_begin == 0 && t_end == n
+                               ? -1
+                               : 2 * (int64_t)blockIdx.x + (t_begin == 0 ? 1 : 0);
+      decode_part<D, Q8, NT>(a, smem, s_bad, seq, hk, L, seq_tiles(a, L), t_begin, t_end, slot);
+      __syncthreads();  // the merged sums have been read
+    }
+    at += p_end - p_begin;
   }
 }
 
@@ -609,14 +620,13 @@ __global__ void __launch_bounds__(128) window_decode_merge_kernel(const Args a) 
   if (n == 0) return;
   const int kvh = h / a.G, j = (h - kvh * a.G) / a.gc, hl = h - kvh * a.G - j * a.gc;
   const int64_t width = a.ws_plan[0];
-  const int64_t first = a.ws_plan[1 + seq] * a.Hk + (int64_t)(kvh * a.hg + j) * n;
+  const int64_t first =  // place of the pair's first tile
+      a.ws_plan[1 + seq] * a.Hk + (int64_t)(kvh * a.hg + j) * places(n) + kOpen;
   const int64_t c0 = first / width;
   const int nsplit = (int)((first + n - 1) / width - c0) + 1;
   if (nsplit == 1) return;  // written whole
-  // range c holds the pair's part in slot 0, but in slot 1 where the pair begins inside it
-  auto part = [&](int s) -> int64_t {
-    return (2 * (c0 + s) + ((c0 + s) * width < first ? 1 : 0)) * a.gc + hl;
-  };
+  // the pair's first part is the last of its range (slot 1), the others their range's first
+  auto part = [&](int s) -> int64_t { return (2 * (c0 + s) + (s == 0 ? 1 : 0)) * a.gc + hl; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // every warp finds the common maximum, 32 ranges at a time
   float M = -INFINITY;
@@ -681,7 +691,7 @@ Plan make_plan(int64_t num_seqs, int Hq, int Hkv, int D, int64_t max_len, int wi
   const int64_t tiles = (keys + kKeys - 1) / kKeys + 2;
   const int64_t units = num_seqs * Hkv * p.hg, slots = (int64_t)kMaxPerSm * va_host::sm_count();
   if (tiles <= 2 * kMinRange || units >= 16 * slots) return p;
-  const int64_t most = units * ((tiles + kMinRange - 1) / kMinRange);
+  const int64_t most = units * ((tiles + kOpen + kMinRange - 1) / kMinRange);
   p.most = (int)(most < slots ? most : slots);
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   p.o_ml = up((size_t)p.most * 2 * p.gc * D * 4);
