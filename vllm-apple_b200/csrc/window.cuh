@@ -97,6 +97,7 @@ inline bool rows_ok(const void *p, int64_t s_token, int64_t s_head) {
 inline bool head_size_ok(int D) { return D == 32 || D == 64 || D == 96 || D == 128; }
 // Positions stay below INT32_MAX / 2, so a window past that is none.
 inline int window_of(int window) { return window > 0 && window < INT32_MAX / 2 ? window : 0; }
+inline int sinks_of(int sinks) { return sinks < INT32_MAX / 2 ? sinks : INT32_MAX / 2; }
 // Opts a kernel in to `bytes` of dynamic shared memory, once per device (bit d of `done`;
 // two threads setting it at once is harmless).
 template <typename K>

@@ -685,6 +685,7 @@ Plan make_plan(int64_t num_seqs, int Hq, int Hkv, int D, int64_t max_len, int wi
   p.hg = (G + 15) / 16;
   p.gc = (G + p.hg - 1) / p.hg;
   window = win::window_of(window);
+  sinks = win::sinks_of(sinks);
   int64_t keys = max_len;
   if (window > 0 && (int64_t)window + sinks < keys) keys = (int64_t)window + sinks;
   // an unaligned run and the sinks each reach into one more tile
@@ -814,7 +815,7 @@ extern "C" int va_window_decode(void *out, const void *q, void *k_cache, void *v
   a.gc = p.gc;
   a.bs = win::fast_div(block_size);
   a.window = win::window_of(window);
-  a.sinks = sink_tokens;
+  a.sinks = win::sinks_of(sink_tokens);
   a.ranges = p.most;
   a.B = (int)num_seqs;
   a.Hk = num_kv_heads * p.hg;

@@ -7,16 +7,15 @@
 // group and both tiles; the tiles' keys are the pair's key tiles of 128 (window.cuh), and
 // nothing outside the window and the sinks is read or multiplied.
 //   * warps 0-7: softmax, one thread per row (TMEM lane = row), warps 0-3 tile 0 and 4-7
-//     tile 1.  S comes from TMEM twice, 64 columns at a time (the row maximum, then the
-//     powers), so a row's 128 scores never sit in registers at once.  P goes back over S
-//     as fp16 and feeds the second product from TMEM.  The maximum a row's powers are
-//     taken against only moves when it grows by more than 2^8, so O is rarely rescaled.
-//   * warp 8: issues tcgen05.mma for both tiles in turn -- PV_0(j-1), S_0(j), PV_1(j-1),
-//     S_1(j) -- so one tile's products run while the other tile is in its softmax.
-//   * warps 9-12: bring K and V key tiles into a ring of shared-memory slots in the
-//     128-byte-swizzled layout of the tensor core.  fp16 rows go by 16-byte cp.async; e4m3
-//     rows are loaded one key tile ahead into registers, turned into fp16 (exactly) and
-//     stored.  Row addresses come from the block table once per key tile, so any block
+//     tile 1.  A row's 128 scores sit in the thread's registers (the other warps hand
+//     theirs over with setmaxnreg); P goes back over S as fp16 and feeds the second product
+//     from TMEM.  The maximum a row's powers are taken against only moves when it grows by
+//     more than 2^8, so O is rarely rescaled.
+//   * warp 8, one thread: issues tcgen05.mma for both tiles in turn -- PV_0(j-1), S_0(j),
+//     PV_1(j-1), S_1(j) -- so one tile's products run while the other is in its softmax.
+//   * warps 12-15: bring K and V key tiles into a ring of shared-memory slots in the
+//     128-byte-swizzled layout of the tensor core.  fp16 rows go there by 16-byte cp.async;
+//     e4m3 rows go to a raw buffer first and are turned into fp16 (exactly) from there.  Row addresses come from the block table once per key tile, so any block
 //     size and any strides work; keys that no row of the pair sees are zeros, unread.
 // A key masked for one row but seen by another may hold an infinity or a NaN in V, and
 // 0 * inf would reach the masked row.  In key tiles that are masked in part (at most a
@@ -37,17 +36,28 @@ constexpr int kRows = 128, kKeys = 128, kTiles = 2;
 constexpr int kSoftmax = kTiles * kRows;
 constexpr int kMmaWarp = kSoftmax / 32;
 constexpr int kProducers = 128;
-constexpr int kThreads = kSoftmax + 32 + kProducers;
+constexpr int kFirstProducer = kSoftmax + 128;  // warps 9-11 only lend their registers
+constexpr int kThreads = kFirstProducer + kProducers;
+// Registers: 512 threads launch with 128 each, the whole file; two warpgroups give up 64 a
+// thread and the softmax warpgroups take them: 2 x 128 x (192 + 64) = 512 x 128.
+constexpr int kRegsLaunch = 128, kRegsSoftmax = 192, kRegsOther = 64;
+static_assert(kThreads * kRegsLaunch == 65536 &&
+                  kSoftmax * kRegsSoftmax + (kThreads - kSoftmax) * kRegsOther == 65536,
+              "register shares");
 constexpr int kLag = 2;  // fp16 copies in flight behind the newest
 constexpr uint32_t kWaitLimit = 1u << 22;
+constexpr uint32_t kTmemO = kTiles * kKeys;  // TMEM: S of both tiles, then O of both
 
-template <int D>
+template <int D, bool Q8>
 struct Shape {
   static constexpr int NB = (D + 63) / 64;            // 64-column blocks of a row
   static constexpr uint32_t kTileBytes = NB * 128 * 128;
-  static constexpr int kSlots = NB == 2 ? 5 : 8;      // K/V key tiles in flight
+  // fp16 key tiles of K or V; an e4m3 cache keeps two more as they come
+  static constexpr int kSlots = NB == 2 ? (Q8 ? 4 : 5) : 8;
+  static constexpr uint32_t kRawBytes = Q8 ? kKeys * D : 0;
   static constexpr uint32_t oSlot = kTiles * kTileBytes;
-  static constexpr uint32_t oInfo = oSlot + kSlots * kTileBytes;  // int2 [128] {block, offset}
+  static constexpr uint32_t oRaw = oSlot + kSlots * kTileBytes;
+  static constexpr uint32_t oInfo = oRaw + 2 * kRawBytes;  // int64 [128] row offsets
   static constexpr uint32_t oExp = oInfo + 128 * 8;   // uchar2 [2][128] exponents of K, V
   static constexpr uint32_t oBar = oExp + 2 * 128 * 2;
   static constexpr uint32_t kBytes = oBar + 256 + 1024;  // + alignment slack
@@ -60,34 +70,84 @@ struct Args {
   const int32_t *bt, *qsl, *sl;
   int32_t *err;
   int64_t T, max_blocks, num_blocks;
-  int S, Hkv, G, TQ, bs, window, sinks;
+  int S, Hkv, G, TQ, window, sinks;
+  win::FastDiv bs;
   float scale_log2;
   int64_t s_block, s_head, s_token, c_block, c_head, c_token;
   int64_t q_s_token, q_s_head, o_s_token, o_s_head;
 };
 
+// The MMA warp's instructions, issued by the lane with `go` set.  (A branch around them
+// would have every descriptor moved to uniform registers one by one.)
+VA_DEVINL uint32_t elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one;
+}
+VA_DEVINL void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc,
+                       uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(go)
+      : "memory");
+}
+VA_DEVINL void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc,
+                       uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(go)
+      : "memory");
+}
+VA_DEVINL void umma_commit(uint64_t *bar, uint32_t go) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          va::smem_addr(bar)),
+      "r"(go)
+      : "memory");
+}
+
 VA_DEVINL void producer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kProducers) : "memory"); }
 
-// What a pair of tiles reads.
+// What a pair of tiles reads, in key tiles.
 struct Pair {
-  int pmin[kTiles], pmax[kTiles];  // query positions of each tile; pmax < pmin: empty
-  int window, sinks;
+  int n_sink;             // key tiles 0 .. n_sink - 1 hold sinks
+  int first[kTiles], last[kTiles];  // key tiles of each tile's run; last < 0: no rows
+  int full_from[kTiles], full_to[kTiles], full_sink;  // those that every row sees whole
+
+  VA_DEVINL Pair(const int (&pmin)[kTiles], const int (&pmax)[kTiles], int window, int sinks) {
+    n_sink = (sinks + kKeys - 1) / kKeys;
+    full_sink = sinks / kKeys;
+#pragma unroll
+    for (int h = 0; h < kTiles; ++h) {
+      first[h] = win::run_start(pmin[h], window) / kKeys;
+      last[h] = pmax[h] >= 0 ? pmax[h] / kKeys : -1;
+      full_from[h] = (win::run_start(pmax[h], window) + kKeys - 1) / kKeys;
+      full_to[h] = (pmin[h] + 1) / kKeys - 1;
+    }
+  }
   // key tile c holds a key that some row of tile h sees
   VA_DEVINL bool need(int h, int c) const {
-    return c * kKeys <= pmax[h] &&
-           ((c + 1) * kKeys > win::run_start(pmin[h], window) || c * kKeys < sinks);
+    return c <= last[h] && (c >= first[h] || c < n_sink);
   }
   // every row of tile h sees every key of c
   VA_DEVINL bool full(int h, int c) const {
-    return (c + 1) * kKeys - 1 <= pmin[h] &&
-           (window <= 0 || c * kKeys > pmax[h] - window || (c + 1) * kKeys <= sinks);
+    return c <= full_to[h] && (c >= full_from[h] || c < full_sink);
   }
   // masked in part for a tile that reads it
   VA_DEVINL bool partial(int c) const {
     return (need(0, c) && !full(0, c)) || (need(1, c) && !full(1, c));
-  }
-  VA_DEVINL bool sees(int p, int key) const {
-    return key <= p && (window <= 0 || key > p - window || key < sinks);
   }
 };
 
@@ -96,12 +156,12 @@ VA_DEVINL bool not_finite(uint32_t h) { return (h & 0x7c00u) == 0x7c00u; }
 // Whether every block with a key that the query at p sees is a block of the cache.
 __noinline__ __device__ bool blocks_ok(const Args &a, const int32_t *bt, int p) {
   const int lo = win::run_start(p, a.window);
-  for (int b = lo / a.bs; b <= p / a.bs; ++b) {
+  for (int b = a.bs.div(lo); b <= a.bs.div(p); ++b) {
     const int32_t id = __ldg(bt + b);
     if (id < 0 || id >= a.num_blocks) return false;
   }
   const int ns = min(a.sinks, lo);
-  for (int b = 0; b * (int64_t)a.bs < ns; ++b) {
+  for (int b = 0; b * (int64_t)a.bs.d < ns; ++b) {
     const int32_t id = __ldg(bt + b);
     if (id < 0 || id >= a.num_blocks) return false;
   }
@@ -111,13 +171,13 @@ __noinline__ __device__ bool blocks_ok(const Args &a, const int32_t *bt, int p) 
 // Adds the values of V at (key tile c, columns col..col+31) that are not finite and
 // belong to keys that the query at p sees (they are zeros in shared memory).
 template <bool Q8>
-__noinline__ __device__ void add_not_finite(const Args &a, const int32_t *bt, int kvh, int p,
-                                            const Pair &pr, int c, int col, float *o) {
+__noinline__ __device__ void add_not_finite(const Args &a, const int32_t *bt, int kvh, int p, int c,
+                                            int col, float *o) {
   for (int key = c * kKeys; key < (c + 1) * kKeys; ++key) {
-    if (!pr.sees(p, key)) continue;
-    const int32_t blk = __ldg(bt + key / a.bs);
+    if (key > p || (a.window > 0 && key <= p - a.window && key >= a.sinks)) continue;
+    const int32_t blk = __ldg(bt + a.bs.div(key));
     if (blk < 0 || blk >= a.num_blocks) continue;
-    const int64_t row = blk * a.s_block + kvh * a.s_head + (key % a.bs) * a.s_token + col;
+    const int64_t row = blk * a.s_block + kvh * a.s_head + a.bs.mod(key) * a.s_token + col;
     for (int i = 0; i < 32; ++i) {
       if constexpr (Q8) {
         if ((a.vc[row + i] & 0x7f) == 0x7f) o[i] = NAN;
@@ -131,7 +191,7 @@ __noinline__ __device__ void add_not_finite(const Args &a, const int32_t *bt, in
 
 template <int D, bool Q8>
 __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args a) {
-  using S = Shape<D>;
+  using S = Shape<D, Q8>;
   constexpr int NB = S::NB, kSlots = S::kSlots;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   // 128-byte swizzle atoms must sit on 1024-byte boundaries of the shared window
@@ -149,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
   static_assert((2 * kSlots + 3 * kTiles + 2) * 8 + 16 <= 256, "barrier space");
 
   va::pdl_enter();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   // ---- the pair: pairs of sequence s start at index qsl[s] / TP + s (strictly
   // increasing, and far enough apart for ceil(len / TP) pairs), so a binary search finds
   // the sequence.  Last pairs first: the longest contexts of a prompt start first. ----
@@ -170,25 +230,24 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
   const int64_t t0l = t_begin + local * TP;
   if (local < 0 || t0l >= t_end) return;
   const int L = __ldg(a.sl + seq);
-  if (t_begin < 0 || t_end > a.T || (L > 0 && (L + (int64_t)a.bs - 1) / a.bs > a.max_blocks)) {
+  if (t_begin < 0 || t_end > a.T || (L > 0 && a.bs.div(L - 1) >= a.max_blocks)) {
     if (tid == 0 && local == 0 && kvh == 0) va::raise_flag(a.err, VA_FLAG_CTX_OVERFLOW);
     return;
   }
   if (L <= 0) return;
   const int t0 = (int)t0l, nq = min(TP, t_end - t0);
   const int p0 = L - (t_end - t0);  // position of token t0 (may be negative: skipped)
-  Pair pr;
-  pr.window = a.window;
-  pr.sinks = a.sinks;
+  int pmin[kTiles], pmax[kTiles];  // query positions of each tile; pmax < 0: none
 #pragma unroll
   for (int h = 0; h < kTiles; ++h) {
     const int n = min(a.TQ, nq - h * a.TQ);
-    pr.pmin[h] = max(p0 + h * a.TQ, 0);
-    pr.pmax[h] = n > 0 ? p0 + h * a.TQ + n - 1 : -1;
+    pmin[h] = max(p0 + h * a.TQ, 0);
+    pmax[h] = n > 0 ? max(p0 + h * a.TQ + n - 1, -1) : -1;
   }
-  const int plast = max(pr.pmax[0], pr.pmax[1]);
+  const int plast = max(pmax[0], pmax[1]);
   if (plast < 0) return;
-  const int pfirst = pr.pmax[0] >= 0 ? pr.pmin[0] : pr.pmin[1];
+  const int pfirst = pmax[0] >= 0 ? pmin[0] : pmin[1];
+  const Pair pr(pmin, pmax, a.window, a.sinks);
   const win::Tiles tl = win::key_tiles(pfirst, plast, a.window, a.sinks, kKeys);
   const int nch = tl.count;
   const int32_t *bt = a.bt + seq * a.max_blocks;
@@ -212,19 +271,27 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
 
   auto dead = [&]() { return *(volatile int *)&s_dead != 0; };
+  // A wait that runs out gives up for good, and so does one that runs long after another
+  // thread's has: every wait ends, and those that need not wait do not look at s_dead.
+  bool gone = *tmem_slot != 0;  // all 512 columns are this CTA's: its TMEM begins at column 0
   auto wait_bar = [&](uint64_t *bar, uint32_t parity) {
-    if (dead()) return;
-    if (!va::mbar_wait_bounded(bar, parity, kWaitLimit) && atomicExch(&s_dead, 1) == 0)
-      va::raise_flag(a.err, VA_FLAG_WAIT_TIMEOUT);
+    if (gone || va::mbar_try_wait(bar, parity)) return;
+    for (uint32_t i = 1; i < kWaitLimit; ++i) {
+      if (va::mbar_try_wait(bar, parity)) return;
+      if ((i & 255) == 0 && dead()) break;
+    }
+    gone = true;
+    if (atomicExch(&s_dead, 1) == 0) va::raise_flag(a.err, VA_FLAG_WAIT_TIMEOUT);
   };
 
-  if (warp > kMmaWarp) {
+  if (tid >= kFirstProducer) {
     // =================== producers ===================
-    const int pt = tid - kSoftmax - 32;
-    int2 *info = reinterpret_cast<int2 *>(smem + S::oInfo);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    const int pt = tid - kFirstProducer;
+    // element offset of each row of the key tile in the cache; -1: zeros
+    int64_t *info = reinterpret_cast<int64_t *>(smem + S::oInfo);
     uchar2 *exps = reinterpret_cast<uchar2 *>(smem + S::oExp);
     const int klo = win::run_start(pfirst, a.window);
     const int64_t head_off = kvh * a.s_head;
@@ -234,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       const int key = win::tile_at(tl, j) * kKeys + pt;
       // a sink that only a later row's window has passed is inside the run [klo, plast]
       if (key > plast || (key < klo && key >= a.sinks)) return -1;
-      const int32_t b = __ldg(bt + key / a.bs);
+      const int32_t b = __ldg(bt + a.bs.div(key));
       if (b < 0 || b >= a.num_blocks) {
         va::raise_flag(a.err, VA_FLAG_BAD_BLOCK);
         *(volatile int *)&s_bad = 1;
@@ -242,9 +309,16 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       }
       return b;
     };
-    auto off_of = [&](int j) { return (win::tile_at(tl, j) * kKeys + pt) % a.bs; };
-    auto row_base = [&](int2 r) { return r.x * a.s_block + head_off + r.y * a.s_token; };
+    auto off_of = [&](int j) { return a.bs.mod(win::tile_at(tl, j) * kKeys + pt); };
+    auto row_of = [&](int32_t blk, int j) {
+      return blk >= 0 ? blk * a.s_block + head_off + off_of(j) * a.s_token : int64_t(-1);
+    };
     auto slot_of = [&](int item) { return smem + S::oSlot + (item % kSlots) * S::kTileBytes; };
+    // whether the MMAs that read the item's slot before are done (without waiting), and a wait
+    auto is_empty = [&](int item) {
+      return item < kSlots || gone ||
+             va::mbar_try_wait(&bar_empty[item % kSlots], ((item / kSlots) - 1) & 1);
+    };
     auto wait_empty = [&](int item) {
       if (item >= kSlots) wait_bar(&bar_empty[item % kSlots], ((item / kSlots) - 1) & 1);
     };
@@ -256,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
     if constexpr (!Q8) {
       constexpr int P = D / 8;  // 16-byte pieces per row; each thread copies P of a tile
       int32_t blk = block_of(0);
-      // item i: its copies have landed -> scrub (V of a partly masked tile), publish
+      // an item's copies have landed -> scrub (V of a partly masked tile), publish
       auto finish = [&](int item) {
         const int j = item >> 1;
         if ((item & 1) && pr.partial(win::tile_at(tl, j))) {
@@ -280,42 +354,52 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
         }
         publish(item);
       };
+      int done = 0;  // items published
+      // Copies the item into its slot.  At most kLag items stay unpublished behind the newest
+      // one, and none while this thread waits for a slot.
       auto copy = [&](int item) {
-        wait_empty(item);
+        if (!is_empty(item)) {
+          if (item - done == 2) {
+            win::cp_async_wait<1>();
+            finish(done++);
+          }
+          if (item - done == 1) {
+            win::cp_async_wait<0>();
+            finish(done++);
+          }
+          wait_empty(item);
+        }
         const __half *src = reinterpret_cast<const __half *>(item & 1 ? a.vc : a.kc);
         const uint32_t sl = va::smem_addr(slot_of(item));
 #pragma unroll 4
         for (int i = pt; i < kKeys * P; i += kProducers) {
           const int r = i / P, c = i % P;
-          const int2 e = info[r];
-          const bool on = e.x >= 0;
+          const int64_t e = info[r];
           win::cp_async_zfill<16>(sl + tc::sw128_off(r, c * 8, kKeys),
-                                  src + (on ? row_base(e) + c * 8 : 0), on);
+                                  src + (e >= 0 ? e + c * 8 : 0), e >= 0);
         }
         win::cp_async_commit();
+        if (item - done == kLag) {
+          win::cp_async_wait<kLag>();
+          finish(done++);
+        }
       };
 #pragma unroll 1
       for (int j = 0; j < nch; ++j) {
         producer_sync();  // everyone is done with the rows of the tile before
-        info[pt] = make_int2(blk, off_of(j));
+        info[pt] = row_of(blk, j);
         producer_sync();
         blk = block_of(j + 1);
         copy(2 * j);
-        if (j > 0) {
-          win::cp_async_wait<kLag>();
-          finish(2 * j - kLag);
-        }
         copy(2 * j + 1);
-        if (j > 0) {
-          win::cp_async_wait<kLag>();
-          finish(2 * j + 1 - kLag);
-        }
       }
       win::cp_async_wait<0>();
-      finish(2 * nch - 2);
-      finish(2 * nch - 1);
+      while (done < 2 * nch) finish(done++);
     } else {
+      // The codes of an item come by cp.async into one of two raw buffers, an item ahead;
+      // each thread turns the pieces it copied itself into fp16 in the item's slot.
       constexpr int P = D / 16;  // 16-code pieces per row; each thread takes P of a tile
+      unsigned char *raw = smem + S::oRaw;
       int32_t blk0 = block_of(0), blk1 = block_of(1);
       auto load_exps = [&](int32_t blk, int j) {
         uchar2 e = make_uchar2(va::kQ8ExpBias, va::kQ8ExpBias);
@@ -327,24 +411,39 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
         return e;
       };
       uchar2 e0 = load_exps(blk0, 0);
-      auto load = [&](const uint8_t *src, uint4 (&r)[P]) {
-#pragma unroll
+      // rows of key tile j for everyone; the next tile's exponents and block are on their way
+      auto announce = [&](int j) {
+        producer_sync();  // everyone has issued the copies of the tile before
+        info[pt] = row_of(blk0, j);
+        exps[(j & 1) * kKeys + pt] = e0;
+        producer_sync();
+        blk0 = blk1;
+        if (j + 1 < nch) e0 = load_exps(blk0, j + 1);
+        blk1 = block_of(j + 2);
+      };
+      auto fetch = [&](int item) {
+        const uint8_t *src = item & 1 ? a.vc : a.kc;
+        const uint32_t to = va::smem_addr(raw + (item & 1) * S::kRawBytes);
+#pragma unroll 4
         for (int k = 0; k < P; ++k) {
           const int i = pt + k * kProducers, row = i / P, c = i % P;
-          const int2 e = info[row];
-          r[k] = make_uint4(0, 0, 0, 0);
-          if (e.x >= 0) r[k] = __ldg(reinterpret_cast<const uint4 *>(src + row_base(e) + c * 16));
+          const int64_t e = info[row];
+          win::cp_async_zfill<16>(to + i * 16, src + (e >= 0 ? e + c * 16 : 0), e >= 0);
         }
+        win::cp_async_commit();
       };
-      auto store = [&](int item, uint4 (&r)[P], bool scrub) {
+      auto convert = [&](int item) {
+        const unsigned char *from = raw + (item & 1) * S::kRawBytes;
         unsigned char *sl = slot_of(item);
         const uchar2 *ex = exps + ((item >> 1) & 1) * kKeys;
+        const bool scrub = (item & 1) && pr.partial(win::tile_at(tl, item >> 1));
         bool hit = false;
-#pragma unroll
+#pragma unroll 4
         for (int k = 0; k < P; ++k) {
           const int i = pt + k * kProducers, row = i / P, c = i % P;
+          const uint4 r = *reinterpret_cast<const uint4 *>(from + i * 16);
           const uint32_t f = va::q8_scale_h2(item & 1 ? ex[row].y : ex[row].x);
-          uint32_t w[4] = {r[k].x, r[k].y, r[k].z, r[k].w}, o[8];
+          uint32_t w[4] = {r.x, r.y, r.z, r.w}, o[8];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             if (scrub) {
@@ -363,100 +462,104 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
         if (hit) *(volatile int *)&s_poison = 1;
         publish(item);
       };
-      // rows of key tile j for everyone; the next tile's exponents and block are on their way
-      auto announce = [&](int j) {
-        producer_sync();  // everyone has issued the loads of the tile before
-        info[pt] = make_int2(blk0, j < nch ? off_of(j) : 0);
-        exps[(j & 1) * kKeys + pt] = e0;
-        producer_sync();
-        blk0 = blk1;
-        if (j + 1 < nch) e0 = load_exps(blk0, j + 1);
-        blk1 = block_of(j + 2);
-      };
-      uint4 rk[P], rv[P];
       announce(0);
-      load(a.kc, rk);
+      fetch(0);
+      fetch(1);
 #pragma unroll 1
-      for (int j = 0; j < nch; ++j) {
-        load(a.vc, rv);
-        wait_empty(2 * j);
-        store(2 * j, rk, false);
-        if (j + 1 < nch) {
-          announce(j + 1);
-          load(a.kc, rk);
+      for (int item = 0; item < 2 * nch; ++item) {
+        win::cp_async_wait<1>();
+        wait_empty(item);
+        convert(item);
+        if (item + 2 < 2 * nch) {
+          if ((item & 1) == 0) announce((item >> 1) + 1);
+          fetch(item + 2);
+        } else {
+          win::cp_async_commit();  // keeps the count of groups
         }
-        wait_empty(2 * j + 1);
-        store(2 * j + 1, rv, pr.partial(win::tile_at(tl, j)));
       }
     }
-  } else if (warp == kMmaWarp) {
-    // =================== MMA issue (lane 0) ===================
-    const uint32_t sQ = va::smem_addr(smem), sSlot = sQ + S::oSlot;
-    constexpr uint32_t IDESC_S = tc::idesc_f16(kRows, kKeys, false);
-    constexpr uint32_t IDESC_O = tc::idesc_f16(kRows, NB * 64, true);
-    auto wait_item = [&](int item) {
-      wait_bar(&bar_full[item % kSlots], (item / kSlots) & 1);
+  } else if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == kMmaWarp) {
+      // =================== MMA issue ===================
+      // The whole warp walks the loop, so that the descriptors are uniform values; the one
+      // elected lane issues.
+      const uint32_t one = elect_one();
+      const uint32_t sQ = va::smem_addr(smem);
+      constexpr uint32_t IDESC_S = tc::idesc_f16(kRows, kKeys, false);
+      constexpr uint32_t IDESC_O = tc::idesc_f16(kRows, NB * 64, true);
+      // descriptors differ in their address field (16-byte units) alone
+      const uint64_t dQK = tc::sdesc(sQ, 16, 1024);                   // K-major
+      const uint64_t dV = tc::sdesc(sQ + S::oSlot, kKeys * 128, 1024);  // MN-major: LBO = next
+                                                                      // 64 columns, SBO = 8 keys
+      constexpr uint32_t kTile16 = S::kTileBytes / 16, kSlot16 = S::oSlot / 16;
+      int np[kTiles] = {0, 0};  // PVs issued per tile
+      int sk = 0, sv = kSlots - 1;  // slots of K(j) and V(j-1): items 2j and 2j - 1
+      uint32_t fk = 0, fv = 1;      // phases of their "full" barriers
+      // O_h (+)= P_h V: A = P_h [128 x 128] from TMEM, B = V [128 keys x NB*64]
+      auto issue_pv = [&](int h) {
+        wait_bar(&bar_p[h], np[h] & 1);
+        tc::fence_after_sync();
+        const uint32_t go = gone ? 0 : one, acc = np[h] > 0;
+        const uint64_t v = dV + sv * kTile16;
+#pragma unroll
+        for (int ks = 0; ks < kKeys / 16; ++ks)
+          umma_ts(kTmemO + h * NB * 64, h * 128 + ks * 8, v + ks * 128, IDESC_O, ks ? 1u : acc, go);
+        umma_commit(&bar_o[h], go);
+        ++np[h];
+      };
+      // S_h = Q_h K^T.  It overwrites P_h, read by the PV before it: one thread's
+      // tcgen05.mma run in issue order.
+      auto issue_s = [&](int h) {
+        const uint32_t go = gone ? 0 : one;
+        const uint64_t q = dQK + h * kTile16, k = dQK + kSlot16 + sk * kTile16;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          constexpr uint32_t kBlock16 = 128 * 128 / 16;
+          const uint32_t o = (ks >> 2) * kBlock16 + (ks & 3) * 2;
+          umma_ss(h * 128, q + o, k + o, IDESC_S, ks > 0, go);
+        }
+        umma_commit(&bar_s[h], go);
+      };
+      wait_bar(bar_q, 0);
+      wait_bar(&bar_full[0], 0);
       tc::fence_after_sync();
-    };
-    auto release = [&](int item) {
-      if (lane == 0 && !dead()) tc::umma_commit(&bar_empty[item % kSlots]);
-      __syncwarp();
-    };
-    int np[kTiles] = {0, 0};  // PVs issued per tile
-    wait_bar(bar_q, 0);
+      bool pv0 = pr.need(0, win::tile_at(tl, 0)), pv1 = pr.need(1, win::tile_at(tl, 0));
+      if (pv0) issue_s(0);
+      if (pv1) issue_s(1);
+      umma_commit(&bar_empty[0], gone ? 0 : one);
 #pragma unroll 1
-    for (int j = 0; j <= nch; ++j) {
-      const int c = j < nch ? win::tile_at(tl, j) : 0, cp = j > 0 ? win::tile_at(tl, j - 1) : 0;
-      if (j < nch) wait_item(2 * j);
-      if (j > 0) wait_item(2 * j - 1);
-#pragma unroll
-      for (int h = 0; h < kTiles; ++h) {
-        if (j > 0 && pr.need(h, cp)) {
-          // O_h (+)= P_h V: A = P_h [128 x 128] from TMEM, B = V [128 keys x NB*64] MN-major
-          // (LBO = next 64 columns, SBO = next 8 keys)
-          wait_bar(&bar_p[h], np[h] & 1);
-          if (lane == 0 && !dead()) {
-            tc::fence_after_sync();
-            const uint32_t v = sSlot + ((2 * j - 1) % kSlots) * S::kTileBytes;
-#pragma unroll
-            for (int ks = 0; ks < kKeys / 16; ++ks)
-              tc::umma_f16_ts(tmem + 256 + h * NB * 64, tmem + h * 128 + ks * 8,
-                              tc::sdesc(v + ks * 2048, kKeys * 128, 1024), IDESC_O,
-                              (np[h] > 0 || ks > 0) ? 1u : 0u);
-            tc::umma_commit(&bar_o[h]);
-          }
-          __syncwarp();
-          ++np[h];
+      for (int j = 1; j <= nch; ++j) {
+        // items advance by two
+        sk += 2;
+        sv += 2;
+        if (sk >= kSlots) { sk -= kSlots; fk ^= 1; }
+        if (sv >= kSlots) { sv -= kSlots; fv ^= 1; }
+        const int c = win::tile_at(tl, j);
+        const bool s0 = j < nch && pr.need(0, c), s1 = j < nch && pr.need(1, c);
+        wait_bar(&bar_full[sv], fv);
+        if (pv0) issue_pv(0);
+        if (j < nch) {
+          wait_bar(&bar_full[sk], fk);
+          tc::fence_after_sync();
         }
-        if (h == kTiles - 1 && j > 0) release(2 * j - 1);
-        if (j < nch && pr.need(h, c)) {
-          // S_h = Q_h K^T, K-major operands.  It overwrites P_h, read by the PV before it:
-          // one thread's tcgen05.mma run in issue order.
-          if (lane == 0 && !dead()) {
-            const uint32_t q = sQ + h * S::kTileBytes;
-            const uint32_t k = sSlot + ((2 * j) % kSlots) * S::kTileBytes;
-#pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-              const uint32_t o = (ks >> 2) * 128 * 128 + (ks & 3) * 32;
-              tc::umma_f16(tmem + h * 128, tc::sdesc(q + o, 16, 1024), tc::sdesc(k + o, 16, 1024),
-                           IDESC_S, ks > 0);
-            }
-            tc::umma_commit(&bar_s[h]);
-          }
-          __syncwarp();
-        }
+        if (s0) issue_s(0);
+        if (pv1) issue_pv(1);
+        umma_commit(&bar_empty[sv], gone ? 0 : one);
+        if (s1) issue_s(1);
+        if (j < nch) umma_commit(&bar_empty[sk], gone ? 0 : one);
+        pv0 = s0;
+        pv1 = s1;
       }
-      if (j < nch) release(2 * j);
-    }
-    // every MMA issued above has retired before TMEM is freed
-    if (lane == 0) {
-      tc::umma_commit(bar_end);
+      // every MMA issued above has retired before TMEM is freed
+      umma_commit(bar_end, one);
       if (!va::mbar_wait_bounded(bar_end, 0, kWaitLimit) && atomicExch(&s_dead, 1) == 0)
         va::raise_flag(a.err, VA_FLAG_WAIT_TIMEOUT);
+      __syncwarp();
     }
-    __syncwarp();
   } else {
     // =================== Q, then softmax of tile h, one thread per row ===================
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     const int h = warp >> 2, row = tid & (kRows - 1);
     const int head0 = kvh * a.G;
     {
@@ -479,10 +582,10 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
     const int tk = row / a.G, g = row - tk * a.G, ti = h * a.TQ + tk;
     const bool row_ok = tk < a.TQ && ti < nq && p0 + ti >= 0;
     // rows of no token take the tile's last position: their result is dropped
-    const int pos = row_ok ? p0 + ti : pr.pmax[h];
+    const int pos = row_ok ? p0 + ti : pmax[h];
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tmem + h * 128 + lane_base;
-    const uint32_t tO = tmem + 256 + h * NB * 64 + lane_base;
+    const uint32_t tS = h * 128 + lane_base;
+    const uint32_t tO = kTmemO + h * NB * 64 + lane_base;
     const float sc = a.scale_log2;
     float m = -INFINITY, l = 0.f;
     int n = 0;  // key tiles of this tile so far
@@ -493,45 +596,41 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       // columns [vlo, vhi] and [0, vsk) of the key tile are visible
       const bool masked = !pr.full(h, c);
       const int vhi = pos - c * kKeys;
-      const int vlo = a.window > 0 ? pos - a.window + 1 - c * kKeys : INT_MIN;
+      const int vlo = a.window > 0 ? pos - a.window + 1 - c * kKeys : 0;
       const int vsk = a.sinks - c * kKeys;
       wait_bar(&bar_s[h], n & 1);
       tc::fence_after_sync();
-      auto load64 = [&](int half, float (&p)[64]) {
-        uint32_t x[32], y[32];
-        tc::tmem_ld32(tS + half * 64, x);
-        tc::tmem_ld32(tS + half * 64 + 32, y);
+      float p[kKeys];
+      {
+        uint32_t x[4][32];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) tc::tmem_ld32(tS + k * 32, x[k]);
         tc::tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          p[i] = __uint_as_float(x[i]);
-          p[32 + i] = __uint_as_float(y[i]);
-        }
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            const int k = half * 64 + i;
-            p[i] = k <= vhi && (k >= vlo || k < vsk) ? p[i] : -INFINITY;
-          }
-        }
-      };
-      float rmax = -INFINITY;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float p[64];
-        load64(half, p);
-        float x[4] = {p[0], p[1], p[2], p[3]};
-#pragma unroll
-        for (int i = 4; i < 60; i += 8) {
-          x[0] = tc::fmax3(x[0], p[i], p[i + 1]);
-          x[1] = tc::fmax3(x[1], p[i + 2], p[i + 3]);
-          x[2] = tc::fmax3(x[2], p[i + 4], p[i + 5]);
-          x[3] = tc::fmax3(x[3], p[i + 6], p[i + 7]);
-        }
-        x[0] = tc::fmax3(x[0], p[60], p[61]);
-        x[1] = tc::fmax3(x[1], p[62], p[63]);
-        rmax = fmaxf(rmax, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+        for (int i = 0; i < kKeys; ++i) p[i] = __uint_as_float(x[i >> 5][i & 31]);
       }
+      if (masked) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // bits [vlo, vhi] and [0, vsk) of columns 32k .. 32k + 31
+          auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; };
+          const uint32_t see =
+              below(vhi + 1 - 32 * k) & (~below(vlo - 32 * k) | below(vsk - 32 * k));
+#pragma unroll
+          for (int i = 0; i < 32; ++i) p[32 * k + i] = see >> i & 1 ? p[32 * k + i] : -INFINITY;
+        }
+      }
+      float mx[4] = {p[0], p[1], p[2], p[3]};
+#pragma unroll
+      for (int i = 4; i < kKeys - 4; i += 8) {
+        mx[0] = tc::fmax3(mx[0], p[i], p[i + 1]);
+        mx[1] = tc::fmax3(mx[1], p[i + 2], p[i + 3]);
+        mx[2] = tc::fmax3(mx[2], p[i + 4], p[i + 5]);
+        mx[3] = tc::fmax3(mx[3], p[i + 6], p[i + 7]);
+      }
+      mx[0] = tc::fmax3(mx[0], p[kKeys - 4], p[kKeys - 3]);
+      mx[1] = tc::fmax3(mx[1], p[kKeys - 2], p[kKeys - 1]);
+      float rmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       rmax *= sc;  // the scale is positive
       const float mn = (m == -INFINITY || rmax > m + 8.f) ? fmaxf(m, rmax) : m;
       const bool none = mn == -INFINITY;  // no visible key so far
@@ -557,20 +656,18 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       uint64_t sum2[2] = {tc::pk2(0.f, 0.f), tc::pk2(0.f, 0.f)};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        float p[64];
-        load64(half, p);
         uint32_t w[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
+          const int k = half * 64 + 2 * i;
           float x0, x1;
-          tc::upk2(tc::ffma2(tc::pk2(p[2 * i], p[2 * i + 1]), sc2, nm2), x0, x1);
+          tc::upk2(tc::ffma2(tc::pk2(p[k], p[k + 1]), sc2, nm2), x0, x1);
           x0 = va::fast_exp2(x0);
           x1 = va::fast_exp2(x1);
           sum2[i & 1] = tc::fadd2(sum2[i & 1], tc::pk2(x0, x1));
           w[i] = va::pack_h2(x0, x1);
         }
-        // over S columns that this thread has read already
-        tc::tmem_st32(tS + half * 32, w);
+        tc::tmem_st32(tS + half * 32, w);  // over S, which is in registers
       }
       float y0, y1, y2, y3;
       tc::upk2(sum2[0], y0, y1);
@@ -585,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       wait_bar(&bar_o[h], (n - 1) & 1);
       tc::fence_after_sync();
       const bool poison = *(volatile int *)&s_poison != 0;  // some V value was scrubbed
-      bool write = row_ok && !dead();
+      bool write = row_ok && !gone && !dead();
       if (*(volatile int *)&s_bad != 0) write = write && blocks_ok(a, bt, pos);
       const float inv = 1.f / l;
       __half *orow = a.out + (t0 + ti) * a.o_s_token + (int64_t)(head0 + g) * a.o_s_head;
@@ -603,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
             for (int i = 0; i < 32; ++i) fix[i] = 0.f;
             for (int j = 0; j < nch; ++j) {
               const int c = win::tile_at(tl, j);
-              if (pr.partial(c)) add_not_finite<Q8>(a, bt, kvh, pos, pr, c, k, fix);
+              if (pr.partial(c)) add_not_finite<Q8>(a, bt, kvh, pos, c, k, fix);
             }
             for (int i = 0; i < 32; ++i) o[i] += fix[i];
           }
@@ -621,16 +718,27 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
   __syncthreads();
   if (warp == kMmaWarp) {
     tc::fence_after_sync();
-    tc::tmem_dealloc(tmem, tc::kTmemCols);
+    tc::tmem_dealloc(*tmem_slot, tc::kTmemCols);
   }
 }
 
 template <int D, bool Q8>
 int launch_t(const Args &a, unsigned grid, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
-  if (!win::allow_smem(window_prefill_kernel<D, Q8>, (int)Shape<D>::kBytes, done))
+  static std::atomic<int> regs{0};
+  if (!win::allow_smem(window_prefill_kernel<D, Q8>, (int)Shape<D, Q8>::kBytes, done))
     return VA_ERR_LAUNCH;
-  if (va_host::launch_pdl_smem(window_prefill_kernel<D, Q8>, grid, kThreads, Shape<D>::kBytes, st,
+  // the register shares only add up when the build gave every thread kRegsLaunch: with fewer
+  // the softmax warps would wait for registers for good
+  int r = regs.load(std::memory_order_relaxed);
+  if (!r) {
+    cudaFuncAttributes at;
+    if (cudaFuncGetAttributes(&at, window_prefill_kernel<D, Q8>) != cudaSuccess)
+      return VA_ERR_LAUNCH;
+    regs.store(r = at.numRegs, std::memory_order_relaxed);
+  }
+  if (r != kRegsLaunch) return VA_ERR_LAUNCH;
+  if (va_host::launch_pdl_smem(window_prefill_kernel<D, Q8>, grid, kThreads, Shape<D, Q8>::kBytes, st,
                                a))
     return VA_ERR_LAUNCH;
   return va_host::launch_status();
@@ -688,9 +796,9 @@ extern "C" int va_window_prefill(void *out, const void *q, const void *k_cache,
   a.Hkv = num_kv_heads;
   a.G = G;
   a.TQ = kRows / G;
-  a.bs = block_size;
+  a.bs = win::fast_div(block_size);
   a.window = win::window_of(window);
-  a.sinks = sink_tokens;
+  a.sinks = win::sinks_of(sink_tokens);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.s_block = s_block; a.s_head = s_head; a.s_token = s_token;
   a.c_block = sc_block; a.c_head = sc_head; a.c_token = sc_token;
