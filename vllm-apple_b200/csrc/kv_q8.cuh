@@ -55,6 +55,16 @@ VA_DEVINL uint32_t q8_decode2(uint32_t c) {
   return r;
 }
 
+// Four e4m3 codes as two fp16 pairs.
+VA_DEVINL void q8_decode4(uint32_t c, uint32_t &lo, uint32_t &hi) {
+  asm("{\n\t.reg .b16 l, h;\n\t"
+      "mov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(c));
+}
+
 VA_DEVINL uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));

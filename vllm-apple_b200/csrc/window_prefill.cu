@@ -58,8 +58,8 @@ struct Shape {
   static constexpr uint32_t oSlot = kTiles * kTileBytes;
   static constexpr uint32_t oRaw = oSlot + kSlots * kTileBytes;
   static constexpr uint32_t oInfo = oRaw + 2 * kRawBytes;  // int64 [128] row offsets
-  static constexpr uint32_t oExp = oInfo + 128 * 8;   // uchar2 [2][128] exponents of K, V
-  static constexpr uint32_t oBar = oExp + 2 * 128 * 2;
+  static constexpr uint32_t oExp = oInfo + 128 * 8;  // fp16 scales: K [128], V [2][128]
+  static constexpr uint32_t oBar = oExp + 3 * 128 * 2;
   static constexpr uint32_t kBytes = oBar + 256 + 1024;  // + alignment slack
 };
 
@@ -399,7 +399,12 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       // The codes of an item come by cp.async into one of two raw buffers, an item ahead;
       // each thread turns the pieces it copied itself into fp16 in the item's slot.
       constexpr int P = D / 16;  // 16-code pieces per row; each thread takes P of a tile
-      unsigned char *raw = smem + S::oRaw;
+      // piece k of this thread: row and column; rows a multiple of 8 apart unless P = 6, so
+      // that every address below is one base and a constant
+      auto piece_row = [&](int k) { return P == 6 ? (pt + k * kProducers) / 6 : pt / P + k * (kProducers / P); };
+      auto piece_col = [&](int k) { return P == 6 ? (pt + k * kProducers) % 6 : pt % P; };
+      unsigned char *raw = smem + S::oRaw + pt * 16;
+      __half *scale_k = reinterpret_cast<__half *>(smem + S::oExp), *scale_v = scale_k + kKeys;
       int32_t blk0 = block_of(0), blk1 = block_of(1);
       auto load_exps = [&](int32_t blk, int j) {
         uchar2 e = make_uchar2(va::kQ8ExpBias, va::kQ8ExpBias);
@@ -411,11 +416,13 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
         return e;
       };
       uchar2 e0 = load_exps(blk0, 0);
-      // rows of key tile j for everyone; the next tile's exponents and block are on their way
+      // rows of key tile j for everyone (offset | 1; 0: zeros) and their scales; the next
+      // tile's exponents and block are on their way
       auto announce = [&](int j) {
-        producer_sync();  // everyone has issued the copies of the tile before
-        info[pt] = row_of(blk0, j);
-        exps[(j & 1) * kKeys + pt] = e0;
+        producer_sync();  // K(j-1) is converted, V(j-1) on its way
+        info[pt] = blk0 >= 0 ? row_of(blk0, j) | 1 : 0;
+        scale_k[pt] = __ushort_as_half((unsigned short)va::q8_scale_h2(e0.x));
+        scale_v[(j & 1) * kKeys + pt] = __ushort_as_half((unsigned short)va::q8_scale_h2(e0.y));
         producer_sync();
         blk0 = blk1;
         if (j + 1 < nch) e0 = load_exps(blk0, j + 1);
@@ -424,40 +431,45 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       auto fetch = [&](int item) {
         const uint8_t *src = item & 1 ? a.vc : a.kc;
         const uint32_t to = va::smem_addr(raw + (item & 1) * S::kRawBytes);
-#pragma unroll 4
+#pragma unroll
         for (int k = 0; k < P; ++k) {
-          const int i = pt + k * kProducers, row = i / P, c = i % P;
-          const int64_t e = info[row];
-          win::cp_async_zfill<16>(to + i * 16, src + (e >= 0 ? e + c * 16 : 0), e >= 0);
+          const int64_t e = info[piece_row(k)];
+          win::cp_async_zfill<16>(to + k * kProducers * 16, src + (e & ~int64_t(15)) + piece_col(k) * 16,
+                                  e & 1);
         }
         win::cp_async_commit();
       };
       auto convert = [&](int item) {
         const unsigned char *from = raw + (item & 1) * S::kRawBytes;
         unsigned char *sl = slot_of(item);
-        const uchar2 *ex = exps + ((item >> 1) & 1) * kKeys;
+        const __half *scale = item & 1 ? scale_v + (item >> 1 & 1) * kKeys : scale_k;
         const bool scrub = (item & 1) && pr.partial(win::tile_at(tl, item >> 1));
-        bool hit = false;
-#pragma unroll 4
-        for (int k = 0; k < P; ++k) {
-          const int i = pt + k * kProducers, row = i / P, c = i % P;
-          const uint4 r = *reinterpret_cast<const uint4 *>(from + i * 16);
-          const uint32_t f = va::q8_scale_h2(item & 1 ? ex[row].y : ex[row].x);
-          uint32_t w[4] = {r.x, r.y, r.z, r.w}, o[8];
+        uint32_t hit = 0;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            if (scrub) {
+        for (int k = 0; k < P; ++k) {
+          const uint4 r = *reinterpret_cast<const uint4 *>(from + k * kProducers * 16);
+          const uint32_t f = (uint32_t)__half_as_ushort(scale[piece_row(k)]) * 0x10001u;
+          uint32_t w[4] = {r.x, r.y, r.z, r.w}, o[8];
+          if (scrub) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
               const uint32_t bad = __vcmpeq4(w[x] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-              hit = hit || bad;
+              hit |= bad;
               w[x] &= ~bad;
             }
-            o[2 * x] = va::hmul2(va::q8_decode2(w[x]), f);
-            o[2 * x + 1] = va::hmul2(va::q8_decode2(w[x] >> 16), f);
           }
-          *reinterpret_cast<uint4 *>(sl + tc::sw128_off(row, c * 16, kKeys)) =
-              make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4 *>(sl + tc::sw128_off(row, c * 16 + 8, kKeys)) =
-              make_uint4(o[4], o[5], o[6], o[7]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            va::q8_decode4(w[x], o[2 * x], o[2 * x + 1]);
+            o[2 * x] = va::hmul2(o[2 * x], f);
+            o[2 * x + 1] = va::hmul2(o[2 * x + 1], f);
+          }
+          // 16-byte chunks 2c, 2c + 1 of the row; the first one's place differs by bit 4
+          const uint32_t to = P == 6 ? tc::sw128_off(piece_row(k), piece_col(k) * 16, kKeys)
+                                     : tc::sw128_off(pt / P, pt % P * 16, kKeys) +
+                                           k * (kProducers / P) * 128;
+          *reinterpret_cast<uint4 *>(sl + to) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4 *>(sl + (to ^ 16)) = make_uint4(o[4], o[5], o[6], o[7]);
         }
         if (hit) *(volatile int *)&s_poison = 1;
         publish(item);
