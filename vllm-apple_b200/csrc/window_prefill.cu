@@ -71,7 +71,7 @@ struct Args {
   int32_t *err;
   int64_t T, max_blocks, num_blocks;
   int S, Hkv, G, TQ, window, sinks;
-  win::FastDiv bs;
+  win::FastDiv bs, g;
   float scale_log2;
   int64_t s_block, s_head, s_token, c_block, c_head, c_token;
   int64_t q_s_token, q_s_head, o_s_token, o_s_head;
@@ -137,7 +137,8 @@ struct Pair {
       full_to[h] = (pmin[h] + 1) / kKeys - 1;
     }
   }
-  // key tile c holds a key that some row of tile h sees
+  // key tile c holds a key that some row of tile h sees (h known at compile time, so that
+  // nothing here is an indexed array)
   VA_DEVINL bool need(int h, int c) const {
     return c <= last[h] && (c >= first[h] || c < n_sink);
   }
@@ -290,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
     // =================== producers ===================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
     const int pt = tid - kFirstProducer;
-    // element offset of each row of the key tile in the cache; -1: zeros
+    // element offset of each row of the key tile in the cache, | 1; 0: zeros
     int64_t *info = reinterpret_cast<int64_t *>(smem + S::oInfo);
     uchar2 *exps = reinterpret_cast<uchar2 *>(smem + S::oExp);
     const int klo = win::run_start(pfirst, a.window);
@@ -310,8 +311,9 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       return b;
     };
     auto off_of = [&](int j) { return a.bs.mod(win::tile_at(tl, j) * kKeys + pt); };
+    // (offsets are multiples of 8)
     auto row_of = [&](int32_t blk, int j) {
-      return blk >= 0 ? blk * a.s_block + head_off + off_of(j) * a.s_token : int64_t(-1);
+      return blk >= 0 ? (blk * a.s_block + head_off + off_of(j) * a.s_token) | 1 : int64_t(0);
     };
     auto slot_of = [&](int item) { return smem + S::oSlot + (item % kSlots) * S::kTileBytes; };
     // whether the MMAs that read the item's slot before are done (without waiting), and a wait
@@ -329,23 +331,31 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
 
     if constexpr (!Q8) {
       constexpr int P = D / 8;  // 16-byte pieces per row; each thread copies P of a tile
+      // piece k of this thread: row, column and place in a slot; rows a multiple of 8 apart
+      // unless P = 12, so that the places are one base and a constant
+      auto piece_row = [&](int k) { return P == 12 ? (pt + k * kProducers) / 12 : pt / P + k * (kProducers / P); };
+      auto piece_col = [&](int k) { return P == 12 ? (pt + k * kProducers) % 12 : pt % P; };
+      const uint32_t place0 = tc::sw128_off(pt / P, pt % P * 8, kKeys);
+      auto place = [&](int k) {
+        return P == 12 ? tc::sw128_off(piece_row(k), piece_col(k) * 8, kKeys)
+                       : place0 + k * (kProducers / P) * 128;
+      };
       int32_t blk = block_of(0);
       // an item's copies have landed -> scrub (V of a partly masked tile), publish
       auto finish = [&](int item) {
-        const int j = item >> 1;
-        if ((item & 1) && pr.partial(win::tile_at(tl, j))) {
+        if ((item & 1) && pr.partial(win::tile_at(tl, item >> 1))) {
           unsigned char *sl = slot_of(item);
           bool hit = false;
 #pragma unroll 4
-          for (int i = pt; i < kKeys * P; i += kProducers) {
-            uint4 *w = reinterpret_cast<uint4 *>(sl + tc::sw128_off(i / P, (i % P) * 8, kKeys));
+          for (int k = 0; k < P; ++k) {
+            uint4 *w = reinterpret_cast<uint4 *>(sl + place(k));
             uint32_t x[4] = {w->x, w->y, w->z, w->w};
-            bool h = false;
+            uint32_t h = 0;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t bad = __vcmpgeu2(x[k] & 0x7fff7fffu, 0x7c007c00u);
-              h = h || bad;
-              x[k] &= ~bad;
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t bad = __vcmpgeu2(x[i] & 0x7fff7fffu, 0x7c007c00u);
+              h |= bad;
+              x[i] &= ~bad;
             }
             if (h) *w = make_uint4(x[0], x[1], x[2], x[3]);
             hit = hit || h;
@@ -371,12 +381,10 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
         }
         const __half *src = reinterpret_cast<const __half *>(item & 1 ? a.vc : a.kc);
         const uint32_t sl = va::smem_addr(slot_of(item));
-#pragma unroll 4
-        for (int i = pt; i < kKeys * P; i += kProducers) {
-          const int r = i / P, c = i % P;
-          const int64_t e = info[r];
-          win::cp_async_zfill<16>(sl + tc::sw128_off(r, c * 8, kKeys),
-                                  src + (e >= 0 ? e + c * 8 : 0), e >= 0);
+#pragma unroll P == 12 ? 4 : P
+        for (int k = 0; k < P; ++k) {
+          const int64_t e = info[piece_row(k)];
+          win::cp_async_zfill<16>(sl + place(k), src + (e & ~int64_t(7)) + piece_col(k) * 8, e & 1);
         }
         win::cp_async_commit();
         if (item - done == kLag) {
@@ -416,11 +424,11 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
         return e;
       };
       uchar2 e0 = load_exps(blk0, 0);
-      // rows of key tile j for everyone (offset | 1; 0: zeros) and their scales; the next
-      // tile's exponents and block are on their way
+      // rows of key tile j and their scales for everyone; the next tile's exponents and block
+      // are on their way
       auto announce = [&](int j) {
         producer_sync();  // K(j-1) is converted, V(j-1) on its way
-        info[pt] = blk0 >= 0 ? row_of(blk0, j) | 1 : 0;
+        info[pt] = row_of(blk0, j);
         scale_k[pt] = __ushort_as_half((unsigned short)va::q8_scale_h2(e0.x));
         scale_v[(j & 1) * kKeys + pt] = __ushort_as_half((unsigned short)va::q8_scale_h2(e0.y));
         producer_sync();
@@ -579,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
 #pragma unroll 4
       for (int i = tid; i < kTiles * kRows * P; i += kSoftmax) {
         const int r2 = i / P, c = i - r2 * P, hh = r2 / kRows, r = r2 - hh * kRows;
-        const int tk = r / a.G, g = r - tk * a.G, ti = hh * a.TQ + tk;
+        const int tk = a.g.div(r), g = r - tk * a.G, ti = hh * a.TQ + tk;
         const bool on = tk < a.TQ && ti < nq;
         win::cp_async_zfill<16>(
             va::smem_addr(smem + hh * S::kTileBytes + tc::sw128_off(r, c * 8, kRows)),
@@ -591,10 +599,10 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       va::fence_proxy_async_smem();
       va::mbar_arrive(bar_q);
     }
-    const int tk = row / a.G, g = row - tk * a.G, ti = h * a.TQ + tk;
+    const int tk = a.g.div(row), g = row - tk * a.G, ti = h * a.TQ + tk;
     const bool row_ok = tk < a.TQ && ti < nq && p0 + ti >= 0;
     // rows of no token take the tile's last position: their result is dropped
-    const int pos = row_ok ? p0 + ti : pmax[h];
+    const int pos = row_ok ? p0 + ti : (h ? pmax[1] : pmax[0]);
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = h * 128 + lane_base;
     const uint32_t tO = kTmemO + h * NB * 64 + lane_base;
@@ -604,9 +612,9 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
 #pragma unroll 1
     for (int j = 0; j < nch; ++j) {
       const int c = win::tile_at(tl, j);
-      if (!pr.need(h, c)) continue;
+      if (!(h ? pr.need(1, c) : pr.need(0, c))) continue;
       // columns [vlo, vhi] and [0, vsk) of the key tile are visible
-      const bool masked = !pr.full(h, c);
+      const bool masked = !(h ? pr.full(1, c) : pr.full(0, c));
       const int vhi = pos - c * kKeys;
       const int vlo = a.window > 0 ? pos - a.window + 1 - c * kKeys : 0;
       const int vsk = a.sinks - c * kKeys;
@@ -807,6 +815,7 @@ extern "C" int va_window_prefill(void *out, const void *q, const void *k_cache,
   a.S = (int)num_seqs;
   a.Hkv = num_kv_heads;
   a.G = G;
+  a.g = win::fast_div(G);
   a.TQ = kRows / G;
   a.bs = win::fast_div(block_size);
   a.window = win::window_of(window);
