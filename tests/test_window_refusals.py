@@ -99,9 +99,10 @@ def test_cache_checks():
     k8, e = torch.zeros(3, 2, 16, 64).to(f8), torch.zeros(3, 2, 16, dtype=torch.uint8)
     k16 = torch.zeros(3, 2, 16, 64, dtype=f16)
     q8, g, sc = _window_cache(k8, k8, e, e, "hnd")
-    assert q8 and (g.num_kv_heads, g.block_size) == (2, 16) and sc == (32, 16, 1)
+    # (blocks, heads, block size, head size, strides of block, head and token)
+    assert q8 and g == (3, 2, 16, 64, 2048, 1024, 64) and sc == (32, 16, 1)
     q8, g, sc = _window_cache(k8, k8, e, e, "nhd")
-    assert (g.num_kv_heads, g.block_size) == (16, 2) and sc == (32, 1, 16)
+    assert g == (3, 16, 2, 64, 2048, 64, 1024) and sc == (32, 1, 16)
     assert not _window_cache(k16, k16, None, None, "hnd")[0]
     with pytest.raises(TypeError, match="float8_e4m3fn"):
         _window_cache(k16.float(), k16.float(), None, None, "hnd")
@@ -128,20 +129,28 @@ def test_cache_checks():
 
 
 def test_new_row_and_table_checks():
-    from vllm_apple_b200.ops import CacheGeom, _new_rows, _table
-    g = CacheGeom(4, 2, 16, 64, 2048, 1024, 64)
+    from vllm_apple_b200.ops import _ints, _new_rows, _table
     x = torch.zeros(3, 2, 64, dtype=torch.float16)
-    assert _new_rows(x, x, g, 3) == (128, 64)
-    for bad in (x[:2], x[:, :1], x[..., :32]):
+    assert _new_rows(x, x, 2, 64, 3) == (128, 64)
+    for bad in (x[:2], x[:, :1], x[..., :32], x.transpose(1, 2)):
         with pytest.raises(ValueError):
-            _new_rows(bad, bad, g, 3)
+            _new_rows(bad, bad, 2, 64, 3)
     with pytest.raises(ValueError):
-        _new_rows(x, None, g, 3)
+        _new_rows(x, None, 2, 64, 3)
+    with pytest.raises(ValueError):
+        _new_rows(x, torch.zeros(3, 4, 64, dtype=torch.float16)[:, ::2], 2, 64, 3)
     with pytest.raises(TypeError):
-        _new_rows(x.float(), x.float(), g, 3)
+        _new_rows(x.float(), x.float(), 2, 64, 3)
+    v = torch.zeros(6, dtype=torch.int32)
+    _ints(v, "v", 6)
+    for bad in (v[:5], v[::2]):
+        with pytest.raises(ValueError):
+            _ints(bad, "v", 6)
+    with pytest.raises(TypeError):
+        _ints(v.long(), "v", 6)
     t = torch.zeros(2, 5, dtype=torch.int32)
     assert _table(t, 2) == 5
-    for bad in (t[:1], t[0]):
+    for bad in (t[:1], t[0], torch.zeros(5, 2, dtype=torch.int32).t()):
         with pytest.raises(ValueError):
             _table(bad, 2)
     with pytest.raises(TypeError):

@@ -400,23 +400,30 @@ def kv_sync_blocks(src_k, src_v, dst_k, dst_v, block_table, seq_lens, src_layout
 # ---------------------------------------------------------------------------
 # 8-bit KV cache and windowed attention
 # ---------------------------------------------------------------------------
+_err_ptrs: dict[int, int] = {}
+
+
 def _launch(dev: int, name: str, *args) -> None:
-    """Call a C entry point with device ``dev`` current (the library launches on the
-    current device; the arguments end with a stream of ``dev``)."""
+    """Call a C entry point on the current stream of device ``dev``, with that device
+    current (the library launches on the current device).  Two arguments are added to
+    ``args``: the device's error word and the stream."""
+    err = _err_ptrs.get(dev)
+    if err is None:
+        err = _err_ptrs[dev] = err_flag(dev).data_ptr()  # the word is never replaced
     fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == dev:
-        status = fn(*args)
+    if torch._C._cuda_getDevice() == dev:
+        status = fn(*args, err, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            status = fn(*args)
+            status = fn(*args, err, torch._C._cuda_getCurrentRawStream(dev))
     if status:
         _lib.check(status, name)
 
 
-def _on(dev: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
+def _on(dev: torch.device, names: str, *tensors) -> None:
+    for i, t in enumerate(tensors):
         if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, the call runs on {dev}")
+            raise ValueError(f"{names.split()[i]} is on {t.device}, the call runs on {dev}")
 
 
 def call_workspace(device: int, kind: str, nbytes: int,
@@ -428,25 +435,29 @@ def call_workspace(device: int, kind: str, nbytes: int,
     at the same time on different streams, so they must not share one."""
     if not nbytes:
         return None
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         st = torch.cuda.current_stream(device) if stream is None else stream
         with torch.cuda.stream(st):
             return torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
+    if stream is None:  # the usual case, without the lock: the entry is only ever replaced
+        ws = _workspaces.get((device, kind, torch._C._cuda_getCurrentRawStream(device)))
+        if ws is not None and ws.numel() >= nbytes:
+            return ws
     return workspace(device, kind, nbytes, stream)
 
 
 def _window_cache(k_cache, v_cache, k_scale, v_scale, layout):
     """(kv_e4m3, geometry, exponent strides in (block, head, token) order) of a cache pair
     that is fp16 (no scales) or e4m3 with its exponent bytes."""
-    q8 = k_cache.dtype == torch.float8_e4m3fn
-    if not q8 and k_cache.dtype != torch.float16:
-        raise TypeError(f"KV cache must be float16 or float8_e4m3fn, got {k_cache.dtype}")
+    dtype, shape, st = k_cache.dtype, k_cache.shape, k_cache.stride()
+    q8 = dtype is torch.float8_e4m3fn
+    if not q8 and dtype is not torch.float16:
+        raise TypeError(f"KV cache must be float16 or float8_e4m3fn, got {dtype}")
     if layout not in ("hnd", "nhd"):
         raise ValueError(f"unknown cache layout {layout!r}")
-    st = k_cache.stride()
-    if k_cache.dim() != 4 or (st[3] != 1 and k_cache.shape[3] > 1):
+    if len(shape) != 4 or (st[3] != 1 and shape[3] > 1):
         raise ValueError("KV cache must be 4-D with a contiguous head_size axis")
-    if v_cache.dtype != k_cache.dtype or v_cache.shape != k_cache.shape or v_cache.stride() != st:
+    if v_cache.dtype is not dtype or v_cache.shape != shape or v_cache.stride() != st:
         raise ValueError("K and V caches differ in type, shape or strides")
     if not q8:
         if k_scale is not None or v_scale is not None:
@@ -456,38 +467,58 @@ def _window_cache(k_cache, v_cache, k_scale, v_scale, layout):
         if k_scale is None or v_scale is None:
             raise ValueError("an e4m3 cache needs k_scale and v_scale")
         for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-            if t.dtype != torch.uint8:
+            if t.dtype is not torch.uint8:
                 raise TypeError(f"{n} must be uint8 (exponent + 127), got {t.dtype}")
-            if t.shape != k_cache.shape[:3]:
+            if t.shape != shape[:3]:
                 raise ValueError(f"{n} must have the cache's first three dimensions "
-                                 f"{tuple(k_cache.shape[:3])}, got {tuple(t.shape)}")
+                                 f"{tuple(shape[:3])}, got {tuple(t.shape)}")
         sc = k_scale.stride()
         if v_scale.stride() != sc:
             raise ValueError("k_scale and v_scale differ in strides")
+    nb, x, y, d = shape
     if layout == "hnd":
-        nb, h, bs, d = k_cache.shape
-        return q8, CacheGeom(nb, h, bs, d, st[0], st[1], st[2]), sc
-    nb, bs, h, d = k_cache.shape
-    return q8, CacheGeom(nb, h, bs, d, st[0], st[2], st[1]), (sc[0], sc[2], sc[1])
+        return q8, (nb, x, y, d, *st[:3]), sc
+    return q8, (nb, y, x, d, st[0], st[2], st[1]), (sc[0], sc[2], sc[1])
 
 
-def _new_rows(new_k, new_v, g: CacheGeom, rows: int):
-    st = _rows3(new_k, "new_k")
-    if new_v is None or _rows3(new_v, "new_v") != st or new_k.shape != new_v.shape:
-        raise ValueError("new_k and new_v differ in shape or strides")
-    if new_k.shape[1:] != (g.num_kv_heads, g.head_size) or new_k.shape[0] < rows:
-        raise ValueError(f"new_k / new_v must be [{rows}, {g.num_kv_heads}, {g.head_size}], "
-                         f"got {tuple(new_k.shape)}")
+def _rows(t, name, heads, head_size, rows):
+    """(token, head) strides of an fp16 [>= rows, heads, head_size] tensor."""
+    shape, st = t.shape, t.stride()
+    if t.dtype is not torch.float16:
+        raise TypeError(f"{name} must be float16, got {t.dtype}")
+    if len(shape) != 3 or st[2] != 1 or shape[1] != heads or shape[2] != head_size or (
+            shape[0] < rows):
+        raise ValueError(f"{name} must be [>= {rows}, {heads}, {head_size}] with contiguous "
+                         f"head_size, got {tuple(shape)} with strides {st}")
+    return st[0], st[1]
+
+
+def _new_rows(new_k, new_v, heads, head_size, rows):
+    if new_k is None or new_v is None:
+        raise ValueError("new_k and new_v go together")
+    st = _rows(new_k, "new_k", heads, head_size, rows)
+    if _rows(new_v, "new_v", heads, head_size, rows) != st:
+        raise ValueError("new_k and new_v differ in strides")
     return st
+
+
+def _ints(t, name, rows):
+    """A contiguous int32 vector of at least ``rows`` entries."""
+    if t.dtype is not torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if not t.is_contiguous() or t.numel() < rows:
+        raise ValueError(f"{name} must be contiguous with at least {rows} entries")
 
 
 def _table(block_table, seqs: int) -> int:
     """Blocks per sequence of a block table with at least ``seqs`` rows."""
-    _i32(block_table, "block_table")
-    if block_table.dim() != 2 or block_table.shape[0] < seqs:
-        raise ValueError(f"block_table must be [>= {seqs}, max_blocks], "
-                         f"got {tuple(block_table.shape)}")
-    return block_table.shape[1]
+    shape = block_table.shape
+    if block_table.dtype is not torch.int32:
+        raise TypeError(f"block_table must be int32, got {block_table.dtype}")
+    if len(shape) != 2 or shape[0] < seqs or not block_table.is_contiguous():
+        raise ValueError(f"block_table must be a contiguous [>= {seqs}, max_blocks], "
+                         f"got {tuple(shape)}")
+    return shape[1]
 
 
 def kv_quant_write_slots(k_cache, v_cache, k_scale, v_scale, new_k, new_v, slot_mapping,
@@ -499,22 +530,21 @@ def kv_quant_write_slots(k_cache, v_cache, k_scale, v_scale, new_k, new_v, slot_
     stands for ``codes * 2 ** (scale - 127)``.  Slot -1 is skipped; live slots must be
     distinct."""
     dev = _dev_index(k_cache)
-    q8, g, sc = _window_cache(k_cache, v_cache, k_scale, v_scale, layout)
+    q8, (nb, h, bs, d, *st), sc = _window_cache(k_cache, v_cache, k_scale, v_scale, layout)
     if not q8:
         raise TypeError("kv_quant_write_slots writes a float8_e4m3fn cache")
-    if slot_mapping.dtype not in (torch.int32, torch.int64) or not slot_mapping.is_contiguous():
+    slot64 = slot_mapping.dtype is torch.int64
+    if not (slot64 or slot_mapping.dtype is torch.int32) or not slot_mapping.is_contiguous():
         raise TypeError("slot_mapping must be a contiguous int32 or int64 tensor")
     T = new_k.shape[0]
-    n_st, n_sh = _new_rows(new_k, new_v, g, T)
+    n_st, n_sh = _new_rows(new_k, new_v, h, d, T)
     if slot_mapping.numel() < T:
         raise ValueError("slot_mapping shorter than the number of tokens")
-    _on(k_cache.device, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale, new_k=new_k,
-        new_v=new_v, slot_mapping=slot_mapping)
+    _on(k_cache.device, "v_cache k_scale v_scale new_k new_v slot_mapping", v_cache, k_scale,
+        v_scale, new_k, new_v, slot_mapping)
     _launch(dev, "va_kv_quant_write_slots", k_cache.data_ptr(), v_cache.data_ptr(),
             k_scale.data_ptr(), v_scale.data_ptr(), new_k.data_ptr(), new_v.data_ptr(),
-            slot_mapping.data_ptr(), int(slot_mapping.dtype == torch.int64), T, g.num_kv_heads,
-            g.head_size, g.block_size, g.num_blocks, g.s_block, g.s_head, g.s_token, *sc, n_st,
-            n_sh, err_flag(dev).data_ptr(), _stream(dev))
+            slot_mapping.data_ptr(), slot64, T, h, d, bs, nb, *st, *sc, n_st, n_sh)
 
 
 def kv_dequant_blocks(src_k, src_v, k_scale, v_scale, dst_k, dst_v, block_table, seq_lens,
@@ -525,28 +555,27 @@ def kv_dequant_blocks(src_k, src_v, k_scale, v_scale, dst_k, dst_v, block_table,
     Block ``block_table[s, i]`` of the source goes to ``dst_block_table[s, i]`` (default:
     the same id) of the destination; rows past a sequence's end stay as they are."""
     dev = _dev_index(src_k)
-    q8, s, sc = _window_cache(src_k, src_v, k_scale, v_scale, src_layout)
+    q8, (nb, h, bs, hd, *st), sc = _window_cache(src_k, src_v, k_scale, v_scale, src_layout)
     if not q8:
         raise TypeError("kv_dequant_blocks reads a float8_e4m3fn cache")
     d = cache_geom(dst_k, dst_layout)
     if cache_geom(dst_v, dst_layout) != d:
         raise ValueError("K and V caches differ in shape or strides")
-    if (s.num_kv_heads, s.block_size, s.head_size) != (d.num_kv_heads, d.block_size, d.head_size):
+    if (h, bs, hd) != (d.num_kv_heads, d.block_size, d.head_size):
         raise ValueError("source and destination caches differ in geometry")
-    _i32(seq_lens, "seq_lens")
     B = seq_lens.numel()
+    _ints(seq_lens, "seq_lens", B)
     mb = _table(block_table, B)
     if dst_block_table is not None:
-        _i32(dst_block_table, "dst_block_table")
+        _table(dst_block_table, B)
         if dst_block_table.shape != block_table.shape:
             raise ValueError("dst_block_table and block_table differ in shape")
-    _on(src_k.device, src_v=src_v, k_scale=k_scale, v_scale=v_scale, dst_k=dst_k, dst_v=dst_v,
-        block_table=block_table, seq_lens=seq_lens, dst_block_table=dst_block_table)
+    _on(src_k.device, "src_v k_scale v_scale dst_k dst_v block_table seq_lens dst_block_table",
+        src_v, k_scale, v_scale, dst_k, dst_v, block_table, seq_lens, dst_block_table)
     _launch(dev, "va_kv_dequant_blocks", src_k.data_ptr(), src_v.data_ptr(), k_scale.data_ptr(),
             v_scale.data_ptr(), dst_k.data_ptr(), dst_v.data_ptr(), block_table.data_ptr(),
-            _ptr(dst_block_table), seq_lens.data_ptr(), B, mb, s.num_kv_heads, s.head_size,
-            s.block_size, s.num_blocks, d.num_blocks, s.s_block, s.s_head, s.s_token, *sc,
-            d.s_block, d.s_head, d.s_token, err_flag(dev).data_ptr(), _stream(dev))
+            _ptr(dst_block_table), seq_lens.data_ptr(), B, mb, h, hd, bs, nb, d.num_blocks, *st,
+            *sc, d.s_block, d.s_head, d.s_token)
 
 
 def paged_window_decode(out, q, k_cache, v_cache, block_table, seq_lens, *, scale, max_seq_len,
@@ -559,36 +588,27 @@ def paged_window_decode(out, q, k_cache, v_cache, block_table, seq_lens, *, scal
     [B, Hkv, D] the new row is written first (quantised for an e4m3 cache).  out/q
     [B, Hq, D]; ``max_seq_len`` >= every seq_len; ``scale`` > 0."""
     dev = _dev_index(q)
-    q8, g, sc = _window_cache(k_cache, v_cache, k_scale, v_scale, layout)
-    q_st, q_sh = _rows3(q, "q")
-    o_st, o_sh = _rows3(out, "out")
-    _i32(seq_lens, "seq_lens")
-    B = q.shape[0] if num_seqs is None else num_seqs
-    Hq, D = q.shape[1], q.shape[2]
-    if D != g.head_size:
-        raise ValueError(f"q head_size {D} != cache head_size {g.head_size}")
-    if out.shape[0] < B or q.shape[0] < B or out.shape[1:] != q.shape[1:]:
-        raise ValueError("out and q differ in shape, or hold fewer rows than num_seqs")
-    if seq_lens.numel() < B:
-        raise ValueError("seq_lens shorter than the number of sequences")
+    q8, (nb, h, bs, d, *st), sc = _window_cache(k_cache, v_cache, k_scale, v_scale, layout)
+    B, Hq, _ = q.shape
+    if num_seqs is not None:
+        B = num_seqs
+    q_st = _rows(q, "q", Hq, d, B)
+    o_st = _rows(out, "out", Hq, d, B)
+    _ints(seq_lens, "seq_lens", B)
     mb = _table(block_table, B)
-    n_st = n_sh = 0
+    n_st = (0, 0)
     if new_k is not None or new_v is not None:
-        if new_k is None:
-            raise ValueError("new_k and new_v go together")
-        n_st, n_sh = _new_rows(new_k, new_v, g, B)
-    _on(q.device, out=out, k_cache=k_cache, v_cache=v_cache, block_table=block_table,
-        seq_lens=seq_lens, k_scale=k_scale, v_scale=v_scale, new_k=new_k, new_v=new_v)
+        n_st = _new_rows(new_k, new_v, h, d, B)
+    _on(q.device, "out k_cache v_cache block_table seq_lens k_scale v_scale new_k new_v", out,
+        k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, new_k, new_v)
     window = max(int(window or 0), 0)
-    nbytes = _lib.load().va_window_decode_workspace_size(B, Hq, g.num_kv_heads, D, max_seq_len,
-                                                         window, sink_tokens)
+    nbytes = _lib.load().va_window_decode_workspace_size(B, Hq, h, d, max_seq_len, window,
+                                                         sink_tokens)
     ws = call_workspace(dev, "window_decode", nbytes)
     _launch(dev, "va_window_decode", out.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), int(q8), block_table.data_ptr(),
-            seq_lens.data_ptr(), _ptr(new_k), _ptr(new_v), B, Hq, g.num_kv_heads, D,
-            g.block_size, mb, max_seq_len, g.num_blocks, float(scale), window, sink_tokens,
-            g.s_block, g.s_head, g.s_token, *sc, q_st, q_sh, o_st, o_sh, n_st, n_sh, _ptr(ws),
-            nbytes, err_flag(dev).data_ptr(), _stream(dev))
+            v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), q8, block_table.data_ptr(),
+            seq_lens.data_ptr(), _ptr(new_k), _ptr(new_v), B, Hq, h, d, bs, mb, max_seq_len, nb,
+            scale, window, sink_tokens, *st, *sc, *q_st, *o_st, *n_st, _ptr(ws), nbytes)
 
 
 def paged_window_prefill(out, q, k_cache, v_cache, block_table, query_start_loc, seq_lens, *,
@@ -602,25 +622,19 @@ def paged_window_prefill(out, q, k_cache, v_cache, block_table, query_start_loc,
     positions before it (0: all) and the first ``sink_tokens``.  Rows of no sequence stay as
     they are."""
     dev = _dev_index(q)
-    q8, g, sc = _window_cache(k_cache, v_cache, k_scale, v_scale, layout)
-    q_st, q_sh = _rows3(q, "q")
-    o_st, o_sh = _rows3(out, "out")
-    _i32(query_start_loc, "query_start_loc")
-    _i32(seq_lens, "seq_lens")
-    T, Hq, D = q.shape
+    q8, (nb, h, bs, d, *st), sc = _window_cache(k_cache, v_cache, k_scale, v_scale, layout)
+    T, Hq, _ = q.shape
     S = query_start_loc.numel() - 1 if num_seqs is None else num_seqs
-    if D != g.head_size:
-        raise ValueError(f"q head_size {D} != cache head_size {g.head_size}")
-    if out.shape != q.shape:
-        raise ValueError("out and q differ in shape")
-    if S < 0 or query_start_loc.numel() < S + 1 or seq_lens.numel() < S:
-        raise ValueError("query_start_loc / seq_lens shorter than the number of sequences")
+    q_st = _rows(q, "q", Hq, d, T)
+    o_st = _rows(out, "out", Hq, d, T)
+    if S < 0:
+        raise ValueError("query_start_loc needs one entry more than there are sequences")
+    _ints(query_start_loc, "query_start_loc", S + 1)
+    _ints(seq_lens, "seq_lens", S)
     mb = _table(block_table, S)
-    _on(q.device, out=out, k_cache=k_cache, v_cache=v_cache, block_table=block_table,
-        query_start_loc=query_start_loc, seq_lens=seq_lens, k_scale=k_scale, v_scale=v_scale)
+    _on(q.device, "out k_cache v_cache block_table query_start_loc seq_lens k_scale v_scale", out,
+        k_cache, v_cache, block_table, query_start_loc, seq_lens, k_scale, v_scale)
     _launch(dev, "va_window_prefill", out.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), int(q8), block_table.data_ptr(),
-            query_start_loc.data_ptr(), seq_lens.data_ptr(), T, S, Hq, g.num_kv_heads, D,
-            g.block_size, mb, g.num_blocks, float(scale), max(int(window or 0), 0), sink_tokens,
-            g.s_block, g.s_head, g.s_token, *sc, q_st, q_sh, o_st, o_sh,
-            err_flag(dev).data_ptr(), _stream(dev))
+            v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), q8, block_table.data_ptr(),
+            query_start_loc.data_ptr(), seq_lens.data_ptr(), T, S, Hq, h, d, bs, mb, nb, scale,
+            max(int(window or 0), 0), sink_tokens, *st, *sc, *q_st, *o_st)
