@@ -24,6 +24,9 @@ What changes, on purpose:
     prefill attends only to the new tokens (:1078-1149).
   * encoder (non-causal) attention runs on the same kernels: the new K/V go to
     a scratch paged cache and every token of a sequence sees all of it.
+  * a layer built with ``window_sink_tokens`` (0 or more) has its ``sliding_window``
+    applied and that many first tokens kept visible; the reference carries a window
+    without applying it, and so does a layer built without that argument.
 """
 from __future__ import annotations
 
@@ -138,6 +141,7 @@ class MetalAttentionMetadata:
     # device-side prefill row metadata, built once per step and shared by every layer
     _prefill_token_to_seq: Optional[torch.Tensor] = None
     _prefill_positions: Optional[torch.Tensor] = None
+    _query_start_loc_dev: Optional[torch.Tensor] = None
 
     @property
     def query_start_loc_cpu(self) -> list:
@@ -150,6 +154,12 @@ class MetalAttentionMetadata:
         if self._seq_lens_cpu is None:
             self._seq_lens_cpu = self.seq_lens.tolist()
         return self._seq_lens_cpu
+
+    def query_start_loc_on(self, device) -> torch.Tensor:
+        """``query_start_loc`` as int32 on ``device``, made once per step."""
+        if self._query_start_loc_dev is None:
+            self._query_start_loc_dev = _i32(self.query_start_loc.to(device))
+        return self._query_start_loc_dev
 
     def prefill_rows(self, device):
         """(token_to_seq, positions) int32 on ``device`` for tokens
@@ -222,7 +232,8 @@ class MetalAttentionImpl(AttentionImpl):
                  kv_cache_dtype: str, logits_soft_cap: Optional[float] = None,
                  attn_type: str = AttentionType.DECODER,
                  kv_sharing_target_layer_name: Optional[str] = None,
-                 sinks: Optional[torch.Tensor] = None) -> None:
+                 sinks: Optional[torch.Tensor] = None,
+                 window_sink_tokens: Optional[int] = None) -> None:
         self.kv_sharing_target_layer_name = kv_sharing_target_layer_name
         self._is_kv_shared = kv_sharing_target_layer_name is not None
         self.num_heads = num_heads
@@ -248,6 +259,19 @@ class MetalAttentionImpl(AttentionImpl):
             raise NotImplementedError("FP8 KV cache is unsupported in METAL_ATTN")
         self.attn_type = attn_type
         self.sinks = sinks
+        # A layer that asks for it (vLLM passes extra keyword arguments of a layer on) has its
+        # sliding window applied, with that many first tokens kept visible (0: none).  Without
+        # it the window is carried and not applied, as in the reference's kernels.
+        self.window_sink_tokens = window_sink_tokens
+        self._window = 0
+        if window_sink_tokens is not None:
+            if window_sink_tokens < 0:
+                raise ValueError("window_sink_tokens must not be negative")
+            if sliding_window is None or sliding_window <= 0:
+                raise ValueError("window_sink_tokens needs a sliding_window")
+            if attn_type in (AttentionType.ENCODER_ONLY, AttentionType.ENCODER):
+                raise NotImplementedError("encoder attention has no sliding window here")
+            self._window = sliding_window
 
     def forward(self, layer, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                 kv_cache: torch.Tensor, attn_metadata: Optional[MetalAttentionMetadata],
@@ -294,10 +318,24 @@ class MetalAttentionImpl(AttentionImpl):
             if write:
                 ops.kv_write_slots(kc, vc, k3[nd:], v3[nd:], md.slot_mapping[nd:T].contiguous(),
                                    layout="nhd")
-            tok, pos = md.prefill_rows(q3.device)
-            ops.paged_prefill(o3[nd:], q3[nd:], kc, vc, bt, tok, pos, scale=self.scale,
-                              layout="nhd", num_seqs=bt.shape[0])
-        if nd:
+            if self._window:
+                # the decode rows are the first nd sequences, one token each
+                ops.paged_window_prefill(o3, q3, kc, vc, bt[nd:],
+                                         md.query_start_loc_on(q3.device)[nd:], sl[nd:],
+                                         scale=self.scale, window=self._window,
+                                         sink_tokens=self.window_sink_tokens, layout="nhd",
+                                         num_seqs=bt.shape[0] - nd)
+            else:
+                tok, pos = md.prefill_rows(q3.device)
+                ops.paged_prefill(o3[nd:], q3[nd:], kc, vc, bt, tok, pos, scale=self.scale,
+                                  layout="nhd", num_seqs=bt.shape[0])
+        if nd and self._window:
+            ops.paged_window_decode(o3[:nd], q3[:nd], kc, vc, bt, sl, scale=self.scale,
+                                    max_seq_len=max(int(md.max_seq_len), 1),
+                                    window=self._window, sink_tokens=self.window_sink_tokens,
+                                    new_k=k3[:nd] if write else None,
+                                    new_v=v3[:nd] if write else None, layout="nhd", num_seqs=nd)
+        elif nd:
             ops.paged_decode(o3[:nd], q3[:nd], kc, vc, bt, sl, scale=self.scale,
                              max_seq_len=max(int(md.max_seq_len), 1),
                              new_k=k3[:nd] if write else None, new_v=v3[:nd] if write else None,

@@ -120,3 +120,56 @@ class EngineKVCache:
 
     def get_total_memory_bytes(self) -> int:
         return sum(t.numel() * 2 for t in self._k + self._v)
+
+
+class EngineQuantKVCache(EngineKVCache):
+    """An :class:`EngineKVCache` in 8 bits: per layer one K and one V buffer of e4m3 codes
+    [num_blocks, num_kv_heads, block_size, head_size] and one exponent byte per row
+    ([num_blocks, num_kv_heads, block_size], e + 127).  A row stands for
+    ``codes * 2 ** e``; zero-filled buffers stand for zeros.  About half the memory of the
+    fp16 cache (head_size + 1 bytes a row instead of 2 * head_size)."""
+
+    def __init__(self, engine_context, descriptor: KVCacheDescriptor):
+        self._context = engine_context
+        self._desc = d = descriptor
+        dev = engine_context.device
+        rows = (d.num_blocks, d.num_kv_heads, d.block_size)
+
+        def codes():
+            t = torch.zeros(rows + (d.head_size,), dtype=torch.uint8, device=dev)
+            return t.view(torch.float8_e4m3fn)
+
+        layers = range(d.num_layers)
+        self._k, self._v = [codes() for _ in layers], [codes() for _ in layers]
+        # exponent 0: any exponent of the format does for rows of zeros
+        self._ks, self._vs = ([torch.full(rows, 127, dtype=torch.uint8, device=dev)
+                               for _ in layers] for _ in range(2))
+
+    def get_scale_buffers(self, layer_idx: int):
+        return self._ks[layer_idx], self._vs[layer_idx]
+
+    def read_back(self, layer_idx: int, dst_k, dst_v, block_table, seq_lens,
+                  dst_block_table=None, dst_layout: str = "hnd") -> None:
+        """Copy the active rows of one layer into an fp16 cache, exactly."""
+        from .. import ops
+        dev = dst_k.device
+
+        def ints(t):
+            return None if t is None else t.to(device=dev, dtype=torch.int32).contiguous()
+
+        ops.kv_dequant_blocks(self._k[layer_idx], self._v[layer_idx], self._ks[layer_idx],
+                              self._vs[layer_idx], dst_k, dst_v, ints(block_table),
+                              ints(seq_lens), dst_block_table=ints(dst_block_table),
+                              dst_layout=dst_layout)
+
+    def sync_from_torch_cache(self, torch_caches, block_table, seq_lens) -> None:
+        raise NotImplementedError("an e4m3 cache is written row by row (KVQuantOp.encode_write)")
+
+    def reset(self) -> None:
+        for t in self._k + self._v:
+            t.view(torch.uint8).zero_()
+        for t in self._ks + self._vs:
+            t.fill_(127)
+
+    def get_total_memory_bytes(self) -> int:
+        return sum(t.numel() for t in self._k + self._v + self._ks + self._vs)

@@ -10,6 +10,10 @@ sm_100a kernels on the step's stream (no waits).
   EngineRMSNorm         vllm_apple/engine/ops/rmsnorm.py:176-340
   EngineRoPE            vllm_apple/engine/ops/elementwise.py:610-766
   EngineElementwiseOps  vllm_apple/engine/ops/elementwise.py (encode_silu_mul :496-532)
+
+Two classes have no counterpart there: :class:`WindowedAttentionOp` (attention under a
+sliding window with sinks, over fp16 or e4m3 caches) and :class:`KVQuantOp` (the e4m3
+cache's writes and read-back).
 """
 from __future__ import annotations
 
@@ -248,6 +252,188 @@ class KVWriteOp:
         return {"num_kv_heads": self.num_kv_heads, "head_size": self.head_size,
                 "block_size": self.block_size, "decode_kernel": "va_kv_write_decode",
                 "prefill_kernel": "va_kv_write_slots"}
+
+
+class WindowedAttentionOp:
+    """Paged attention under a sliding window with sinks: a token at position p sees the
+    last ``window`` positions up to its own (0: all) and the first ``sink_tokens``.
+
+    Buffers as in :class:`PagedAttentionOp`; with ``key_scale_buffer`` and
+    ``value_scale_buffer`` (uint8 [num_blocks, num_kv_heads, block_size]) the KV cache is
+    e4m3, see :class:`~vllm_apple_b200.engine.EngineQuantKVCache`.  Blocks that hold no
+    visible key are not read: their block-table entries may hold anything.
+    """
+
+    def __init__(self, context: Any, num_kv_heads: int, num_query_heads: int, head_size: int,
+                 block_size: int, scale: Optional[float] = None, window: int = 0,
+                 sink_tokens: int = 0):
+        if num_query_heads % num_kv_heads:
+            raise ValueError("num_query_heads must be a multiple of num_kv_heads")
+        if window < 0 or sink_tokens < 0:
+            raise ValueError("window and sink_tokens must not be negative")
+        self._context = context
+        self.num_kv_heads = num_kv_heads
+        self.num_query_heads = num_query_heads
+        self.head_size = head_size
+        self.block_size = block_size
+        self.scale = scale if scale is not None else 1.0 / (head_size ** 0.5)
+        if not (self.scale > 0 and math.isfinite(self.scale)):
+            raise ValueError("scale must be positive and finite")
+        self.window = window
+        self.sink_tokens = sink_tokens
+        D, H = head_size, num_kv_heads
+        self._cache_strides = (H * block_size * D, block_size * D, D)
+        self._scale_strides = (H * block_size, block_size, 1)
+        self._row_strides = (num_query_heads * D, D)
+        _lib.load()
+
+    def _cache(self, key, value, key_scale, value_scale):
+        """(pointers of K, V and their scales, kv_e4m3, blocks that all of them hold)."""
+        if (key_scale is None) != (value_scale is None):
+            raise ValueError("key_scale_buffer and value_scale_buffer go together")
+        (k, kn), (v, vn) = resolve(key), resolve(value)
+        if key_scale is None:
+            return k, v, None, None, 0, min(kn, vn) // (self._cache_strides[0] * _H)
+        (ks, ksn), (vs, vsn) = resolve(key_scale), resolve(value_scale)
+        blocks = min(min(kn, vn) // self._cache_strides[0], min(ksn, vsn) // self._scale_strides[0])
+        return k, v, ks, vs, 1, blocks
+
+    def encode_decode_fused(self, step_ctx, query_buffer, new_keys_buffer, new_values_buffer,
+                            key_buffer, value_buffer, block_table_buffer, seq_lens_buffer,
+                            output_buffer, num_seqs: int, max_seq_len: int,
+                            max_blocks_per_seq: int = 0, query_offset: int = 0,
+                            new_keys_offset: int = 0, new_values_offset: int = 0,
+                            output_offset: int = 0, key_scale_buffer=None,
+                            value_scale_buffer=None) -> None:
+        """Write each sequence's new K/V row (quantised for an e4m3 cache) at position
+        seq_len-1 and attend over its visible keys."""
+        nk = resolve(new_keys_buffer, new_keys_offset)[0]
+        nv = resolve(new_values_buffer, new_values_offset)[0]
+        self._decode(step_ctx, query_buffer, query_offset, nk, nv, key_buffer, value_buffer,
+                     block_table_buffer, seq_lens_buffer, output_buffer, output_offset, num_seqs,
+                     max_seq_len, max_blocks_per_seq, key_scale_buffer, value_scale_buffer)
+
+    def encode_decode(self, step_ctx, query_buffer, key_buffer, value_buffer,
+                      block_table_buffer, seq_lens_buffer, output_buffer, num_seqs: int,
+                      max_seq_len: int, max_blocks_per_seq: int = 0, query_offset: int = 0,
+                      output_offset: int = 0, key_scale_buffer=None,
+                      value_scale_buffer=None) -> None:
+        """Decode attention over a cache that already holds the new rows."""
+        self._decode(step_ctx, query_buffer, query_offset, None, None, key_buffer, value_buffer,
+                     block_table_buffer, seq_lens_buffer, output_buffer, output_offset, num_seqs,
+                     max_seq_len, max_blocks_per_seq, key_scale_buffer, value_scale_buffer)
+
+    def _decode(self, step_ctx, qb, qo, nk, nv, kb, vb, btb, slb, ob, oo, num_seqs, max_seq_len,
+                max_blocks, ksb, vsb):
+        step_ctx.require_encoding("encode()")
+        if max_blocks == 0:
+            max_blocks = (max_seq_len + self.block_size - 1) // self.block_size
+        lib = _lib.load()
+        D, Hq, Hkv = self.head_size, self.num_query_heads, self.num_kv_heads
+        k, v, ks, vs, e4m3, blocks = self._cache(kb, vb, ksb, vsb)
+        nbytes = lib.va_window_decode_workspace_size(num_seqs, Hq, Hkv, D, max_seq_len,
+                                                     self.window, self.sink_tokens)
+        ws = _ops.call_workspace(_dev(step_ctx), "window_decode", nbytes, step_ctx.stream)
+        _lib.check(lib.va_window_decode(
+            resolve(ob, oo)[0], resolve(qb, qo)[0], k, v, ks, vs, e4m3, resolve(btb)[0],
+            resolve(slb)[0], nk, nv, num_seqs, Hq, Hkv, D, self.block_size, max_blocks,
+            max_seq_len, blocks, float(self.scale), self.window, self.sink_tokens,
+            *self._cache_strides, *self._scale_strides, *self._row_strides, *self._row_strides,
+            Hkv * D, D, None if ws is None else ws.data_ptr(), nbytes, _err(step_ctx),
+            step_ctx.stream_handle), "va_window_decode")
+        step_ctx.note_dispatch(2 if nbytes else 1)
+
+    def encode_prefill(self, step_ctx, query_buffer, key_buffer, value_buffer,
+                       block_table_buffer, query_start_loc_buffer, seq_lens_buffer,
+                       output_buffer, num_tokens: int, num_seqs: int, max_blocks_per_seq: int,
+                       query_offset: int = 0, output_offset: int = 0, key_scale_buffer=None,
+                       value_scale_buffer=None) -> None:
+        """Causal attention of every sequence's new tokens over its visible keys (K/V already
+        written).  Tokens query_start_loc[s] .. query_start_loc[s+1]-1 are the last ones of
+        sequence s."""
+        step_ctx.require_encoding("encode_prefill()")
+        k, v, ks, vs, e4m3, blocks = self._cache(key_buffer, value_buffer, key_scale_buffer,
+                                                 value_scale_buffer)
+        _lib.check(_lib.load().va_window_prefill(
+            resolve(output_buffer, output_offset)[0], resolve(query_buffer, query_offset)[0], k, v,
+            ks, vs, e4m3, resolve(block_table_buffer)[0], resolve(query_start_loc_buffer)[0],
+            resolve(seq_lens_buffer)[0], num_tokens, num_seqs, self.num_query_heads,
+            self.num_kv_heads, self.head_size, self.block_size, max_blocks_per_seq, blocks,
+            float(self.scale), self.window, self.sink_tokens, *self._cache_strides,
+            *self._scale_strides, *self._row_strides, *self._row_strides, _err(step_ctx),
+            step_ctx.stream_handle), "va_window_prefill")
+        step_ctx.note_dispatch()
+
+    def get_params_dict(self) -> Dict[str, Any]:
+        return {"num_kv_heads": self.num_kv_heads, "num_query_heads": self.num_query_heads,
+                "head_size": self.head_size, "block_size": self.block_size,
+                "scale": self.scale, "window": self.window, "sink_tokens": self.sink_tokens,
+                "kernel": "va_window_decode", "prefill_kernel": "va_window_prefill"}
+
+
+class KVQuantOp:
+    """Writes to and read-back from an e4m3 cache: codes [num_blocks, num_kv_heads,
+    block_size, head_size], one byte each, and exponent bytes [num_blocks, num_kv_heads,
+    block_size] for K and for V."""
+
+    def __init__(self, context: Any, num_kv_heads: int, head_size: int, block_size: int):
+        self._context = context
+        self.num_kv_heads = num_kv_heads
+        self.head_size = head_size
+        self.block_size = block_size
+        self._cache_strides = (num_kv_heads * block_size * head_size, block_size * head_size,
+                               head_size)
+        self._scale_strides = (num_kv_heads * block_size, block_size, 1)
+        _lib.load()
+
+    def _cache(self, *buffers):
+        """Pointers of (K, V, K scales, V scales) and the number of blocks all of them hold."""
+        got = [resolve(b) for b in buffers]
+        blocks = min(min(n for _, n in got[:2]) // self._cache_strides[0],
+                     min(n for _, n in got[2:]) // self._scale_strides[0])
+        return [p for p, _ in got], blocks
+
+    def encode_write(self, step_ctx, new_keys_buffer, new_values_buffer, key_buffer, value_buffer,
+                     key_scale_buffer, value_scale_buffer, slot_mapping_buffer, num_tokens: int,
+                     new_keys_offset: int = 0, new_values_offset: int = 0) -> None:
+        """Quantise fp16 rows and scatter them by slot (int32, or int64 for an int64 buffer;
+        -1 rows are skipped)."""
+        step_ctx.require_encoding("encode_write()")
+        cache, blocks = self._cache(key_buffer, value_buffer, key_scale_buffer,
+                                    value_scale_buffer)
+        is64 = int(buffer_dtype(slot_mapping_buffer) == torch.int64)
+        H, D = self.num_kv_heads, self.head_size
+        _lib.check(_lib.load().va_kv_quant_write_slots(
+            *cache, resolve(new_keys_buffer, new_keys_offset)[0],
+            resolve(new_values_buffer, new_values_offset)[0], resolve(slot_mapping_buffer)[0],
+            is64, num_tokens, H, D, self.block_size, blocks, *self._cache_strides,
+            *self._scale_strides, H * D, D, _err(step_ctx), step_ctx.stream_handle),
+            "va_kv_quant_write_slots")
+        step_ctx.note_dispatch()
+
+    def encode_read(self, step_ctx, key_buffer, value_buffer, key_scale_buffer,
+                    value_scale_buffer, out_key_buffer, out_value_buffer, block_table_buffer,
+                    seq_lens_buffer, num_seqs: int, max_blocks_per_seq: int,
+                    out_block_table_buffer=None) -> None:
+        """Read the active rows back into an fp16 cache of the engine layout, exactly."""
+        step_ctx.require_encoding("encode_read()")
+        cache, blocks = self._cache(key_buffer, value_buffer, key_scale_buffer,
+                                    value_scale_buffer)
+        out = [resolve(b) for b in (out_key_buffer, out_value_buffer)]
+        out_blocks = min(n for _, n in out) // (self._cache_strides[0] * _H)
+        obt = None if out_block_table_buffer is None else resolve(out_block_table_buffer)[0]
+        _lib.check(_lib.load().va_kv_dequant_blocks(
+            *cache, out[0][0], out[1][0], resolve(block_table_buffer)[0], obt,
+            resolve(seq_lens_buffer)[0], num_seqs, max_blocks_per_seq, self.num_kv_heads,
+            self.head_size, self.block_size, blocks, out_blocks, *self._cache_strides,
+            *self._scale_strides, *self._cache_strides, _err(step_ctx), step_ctx.stream_handle),
+            "va_kv_dequant_blocks")
+        step_ctx.note_dispatch()
+
+    def get_params_dict(self) -> Dict[str, Any]:
+        return {"num_kv_heads": self.num_kv_heads, "head_size": self.head_size,
+                "block_size": self.block_size, "write_kernel": "va_kv_quant_write_slots",
+                "read_kernel": "va_kv_dequant_blocks"}
 
 
 class EngineRMSNorm:
