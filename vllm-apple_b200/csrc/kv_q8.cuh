@@ -19,12 +19,13 @@ namespace va {
 
 constexpr int kQ8ExpBias = 127;
 
-// Largest finite |x| of a packed fp16 pair, as fp16 bits per half, folded into `m`
-// (magnitudes of one sign order like their bits).
-VA_DEVINL uint32_t q8_absmax2(uint32_t m, uint32_t w) {
-  uint32_t a = w & 0x7fff7fffu;
-  a &= __vcmpltu2(a, 0x7c007c00u);
-  return __vmaxu2(m, a);
+// Largest |x| of a packed fp16 pair, as fp16 bits per half, folded into `m` (magnitudes of
+// one sign order like their bits; infinities and NaN come out at 0x7c00 and above) ...
+VA_DEVINL uint32_t q8_absmax2(uint32_t m, uint32_t w) { return __vmaxu2(m, w & 0x7fff7fffu); }
+// ... and of the finite ones alone, for the rare row that holds others.
+VA_DEVINL uint32_t q8_absmax2_finite(uint32_t m, uint32_t w) {
+  const uint32_t a = w & 0x7fff7fffu;
+  return __vmaxu2(m, a & __vcmpltu2(a, 0x7c007c00u));
 }
 
 // Exponent of a row whose largest finite magnitude has the fp16 bits `amax`.
@@ -35,16 +36,25 @@ VA_DEVINL int q8_exponent(uint32_t amax) {
   return min(max(e, -14), 7);
 }
 
-VA_DEVINL float q8_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-
 // fp16 bits of 2^e, from the stored byte e + 127 (e in [-14, 7]), in both halves.
 VA_DEVINL uint32_t q8_scale_h2(uint32_t byte) { return ((byte - 112u) << 10 & 0xffffu) * 0x10001u; }
 
-// Two fp16 values times inv (a power of two), as two e4m3 codes (low half -> low byte).
-VA_DEVINL uint32_t q8_encode2(uint32_t h2, float inv) {
-  const float2 f = h2_to_f2(h2);
-  uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(f.y * inv), "f"(f.x * inv));
+// fp16 bits of 2^-e, in both halves.
+VA_DEVINL uint32_t q8_inv_h2(int e) { return (uint32_t)(15 - e) << 10 | (uint32_t)(15 - e) << 26; }
+
+// Four fp16 values times inv (2^-e from q8_inv_h2), as four e4m3 codes.  The product in
+// fp16 is exact wherever it matters: it is at most 512, and what falls below fp16's normal
+// range (2^-14) is below half the smallest code (2^-10) in any case.
+VA_DEVINL uint32_t q8_encode4(uint32_t a, uint32_t b, uint32_t inv) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\t.reg .b32 x, y;\n\t"
+      "mul.rn.f16x2 x, %1, %3;\n\t"
+      "mul.rn.f16x2 y, %2, %3;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 l, x;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f16x2 h, y;\n\t"
+      "mov.b32 %0, {l, h};\n\t}"
+      : "=r"(r)
+      : "r"(a), "r"(b), "r"(inv));
   return r;
 }
 

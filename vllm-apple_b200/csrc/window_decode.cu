@@ -201,19 +201,16 @@ VA_DEVINL void write_new_row(const Args &a, int seq, int kvh, int64_t blk, int o
   if constexpr (!Q8) {
     if (on) *reinterpret_cast<uint4 *>(cache + 2 * dst) = w;
   } else {
-    uint32_t m = va::q8_absmax2(
-        va::q8_absmax2(va::q8_absmax2(va::q8_absmax2(0, w.x), w.y), w.z), w.w);
+    uint32_t m = va::q8_absmax2_finite(
+        va::q8_absmax2_finite(va::q8_absmax2_finite(va::q8_absmax2_finite(0, w.x), w.y), w.z), w.w);
     m = max(m & 0xffffu, m >> 16);
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     const int e = va::q8_exponent(m);
-    const float inv = va::q8_pow2(-e);
-    if (on) {
-      uint2 c;
-      c.x = va::q8_encode2(w.x, inv) | va::q8_encode2(w.y, inv) << 16;
-      c.y = va::q8_encode2(w.z, inv) | va::q8_encode2(w.w, inv) << 16;
-      *reinterpret_cast<uint2 *>(cache + dst) = c;
-    }
+    const uint32_t inv = va::q8_inv_h2(e);
+    if (on)
+      *reinterpret_cast<uint2 *>(cache + dst) =
+          make_uint2(va::q8_encode4(w.x, w.y, inv), va::q8_encode4(w.z, w.w, inv));
     if (sub == 0)
       (is_v ? a.vs : a.ks)[blk * a.c_block + kvh * a.c_head + off * a.c_token] =
           (uint8_t)(e + va::kQ8ExpBias);
