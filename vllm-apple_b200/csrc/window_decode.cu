@@ -72,7 +72,7 @@ struct Args {
   const int32_t *bt, *sl;
   float *ws_acc;     // [2 * ranges][gc][D] un-normalised O of the ranges' first and last parts
   float2 *ws_ml;     // [2 * ranges][gc] (m, l) of them; l < 0: a block could not be read
-  int64_t *ws_plan;  // {places per range, places before sequence 0, 1, ...}
+  int64_t *ws_plan;  // {places per range, open, places before sequence 0, 1, ...}
   int32_t *err;
   int64_t max_blocks, num_blocks, max_len;
   int B, Hq, G, hg, gc, Hk, window, sinks, ranges;
@@ -126,29 +126,37 @@ VA_DEVINL int num_tiles(const Args &a, int L) { return L > 0 ? seq_tiles(a, L).c
 // Fewest tiles of a range: two per warp.
 constexpr int kMinRange = 2 * kNW;
 
-// Beginning a list of tiles (its length, block ids, first copies, the merge of the warps)
-// takes a CTA about as long as this many tiles, so every list counts for that many more
-// when the ranges are cut: its first kOpen places hold no tile.
-constexpr int kOpen = 24;
-VA_DEVINL int places(int tiles) { return tiles > 0 ? tiles + kOpen : 0; }
+// Beginning another list of tiles (its length, block ids, first copies, the merge of the
+// warps) costs a CTA about as long as 28 tiles, so when the ranges are cut every list
+// counts for that many more: its first `open` places hold no tile.  Three quarters of a range at
+// most, since every range begins one list in any case.  Measured at 4, 16, 28 and 48: 128
+// ragged e4m3 contexts 270 (0), 226, 220, 211 and 222 us; 64 shorter ones, whose ranges are
+// some 30 tiles, 29 us (0), 24 (a quarter of a range), 19.5 (three quarters), 23 (28).
+constexpr int kOpenMost = 28;
+VA_DEVINL int places(int tiles, int open) { return tiles > 0 ? tiles + open : 0; }
 
 // The range of this CTA in the list of all places in (sequence, head group, tile) order.
 struct Range {
   int64_t begin, end;  // places of the list
   int64_t before;      // places of one head group before sequence `seq`
   int seq;             // sequence of the first place
+  int open;
 };
-// Every CTA sums the sequences' places for itself (their lengths are few and in L2), so no
+// Every CTA sums the sequences' tiles for itself (their lengths are few and in L2), so no
 // planning kernel runs before; CTA 0 leaves the sums for the merge.
 VA_DEVINL Range find_range(const Args &a) {
   __shared__ int64_t s_warp[kNW];
   __shared__ int64_t s_before;
   __shared__ int s_seq;
+  constexpr int kCount = 17;  // sums hold tiles << 17 | sequences (at most 65535) with tiles
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.B + kNW * 32 - 1) / (kNW * 32);
   const int q0 = min(tid * per, a.B), q1 = min(q0 + per, a.B);
   int64_t mine = 0;
-  for (int q = q0; q < q1; ++q) mine += places(num_tiles(a, seq_len(a, q, blockIdx.x == 0)));
+  for (int q = q0; q < q1; ++q) {
+    const int n = num_tiles(a, seq_len(a, q, blockIdx.x == 0));
+    if (n > 0) mine += (int64_t)n << kCount | 1;
+  }
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -157,29 +165,38 @@ VA_DEVINL Range find_range(const Args &a) {
   }
   if (lane == 31) s_warp[warp] = incl;
   __syncthreads();
-  int64_t total = 0, at = incl - mine;
+  int64_t sum = 0, excl = incl - mine;
 #pragma unroll
   for (int w = 0; w < kNW; ++w) {
-    if (w < warp) at += s_warp[w];
-    total += s_warp[w];
+    if (w < warp) excl += s_warp[w];
+    sum += s_warp[w];
   }
-  total *= a.Hk;
-  const int64_t w = max((total + a.ranges - 1) / a.ranges, (int64_t)kMinRange);
   Range r;
+  r.open = (int)min((sum >> kCount) * a.Hk * 3 / a.ranges / 4, (int64_t)kOpenMost);
+  auto to_places = [&](int64_t x) {
+    return (x >> kCount) + (x & ((1 << kCount) - 1)) * r.open;
+  };
+  const int64_t total = to_places(sum) * a.Hk;
+  const int64_t w = max((total + a.ranges - 1) / a.ranges, (int64_t)kMinRange);
   r.begin = blockIdx.x * w;
   r.end = min(r.begin + w, total);
-  if (r.begin >= at * a.Hk && r.begin < (at + mine) * a.Hk) {  // one thread's sequences hold it
-    int q = q0;
+  int64_t at = to_places(excl);
+  if (r.begin >= at * a.Hk && r.begin < to_places(excl + mine) * a.Hk) {
+    int q = q0;  // this thread's sequences hold the first place
     int64_t x = at;
-    for (int n; x + (n = places(num_tiles(a, seq_len(a, q, false)))) <= r.begin / a.Hk; ++q) x += n;
+    for (int n; x + (n = places(num_tiles(a, seq_len(a, q, false)), r.open)) <= r.begin / a.Hk; ++q)
+      x += n;
     s_before = x;
     s_seq = q;
   }
   if (blockIdx.x == 0) {
-    if (tid == 0) a.ws_plan[0] = w;
+    if (tid == 0) {
+      a.ws_plan[0] = w;
+      a.ws_plan[1] = r.open;
+    }
     for (int q = q0; q < q1; ++q) {
-      a.ws_plan[1 + q] = at;
-      at += places(num_tiles(a, seq_len(a, q, false)));
+      a.ws_plan[2 + q] = at;
+      at += places(num_tiles(a, seq_len(a, q, false)), r.open);
     }
   }
   __syncthreads();
@@ -384,10 +401,8 @@ VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int &s_bad, int s
         for (int x = 0; x < S::KE / 4; ++x) {
           uint32_t a0, a1, a2, a3;
           if constexpr (Q8) {
-            a0 = va::q8_decode2(wa[x]);
-            a2 = va::q8_decode2(wa[x] >> 16);
-            a1 = va::q8_decode2(wb[x]);
-            a3 = va::q8_decode2(wb[x] >> 16);
+            va::q8_decode4(wa[x], a0, a2);
+            va::q8_decode4(wb[x], a1, a3);
           } else {
             a0 = wa[2 * x];
             a2 = wa[2 * x + 1];
@@ -483,10 +498,12 @@ VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int &s_bad, int s
             const uint32_t sel = x & 1 ? 0x7362 : 0x5140;
             const uint32_t p = __byte_perm(w[0][x / 2], w[1][x / 2], sel);
             const uint32_t q = __byte_perm(w[2][x / 2], w[3][x / 2], sel);
-            a0 = va::hmul2(va::q8_decode2(p), f01);
-            a1 = va::hmul2(va::q8_decode2(p >> 16), f01);
-            a2 = va::hmul2(va::q8_decode2(q), f89);
-            a3 = va::hmul2(va::q8_decode2(q >> 16), f89);
+            va::q8_decode4(p, a0, a1);
+            va::q8_decode4(q, a2, a3);
+            a0 = va::hmul2(a0, f01);
+            a1 = va::hmul2(a1, f01);
+            a2 = va::hmul2(a2, f89);
+            a3 = va::hmul2(a3, f89);
           } else {
             a0 = __byte_perm(w[0][x], w[1][x], 0x5410);
             a1 = __byte_perm(w[0][x], w[1][x], 0x7632);
@@ -582,7 +599,7 @@ __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
   int64_t before = r.before;
 #pragma unroll 1
   for (int64_t at = r.begin; at < r.end;) {
-    const int L = seq_len(a, seq, false), n = num_tiles(a, L), np = places(n);
+    const int L = seq_len(a, seq, false), n = num_tiles(a, L), np = places(n, r.open);
     const int64_t rel = at - before * a.Hk;
     if (rel >= (int64_t)np * a.Hk) {  // past this sequence (also where it has no tiles)
       before += np;
@@ -591,7 +608,7 @@ __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
     }
     const int hk = (int)(rel / np), p_begin = (int)(rel - (int64_t)hk * np);
     const int p_end = (int)min((int64_t)np, p_begin + (r.end - at));
-    const int t_begin = max(p_begin - kOpen, 0), t_end = max(p_end - kOpen, 0);
+    const int t_begin = max(p_begin - r.open, 0), t_end = max(p_end - r.open, 0);
     if (t_end > t_begin) {
       // a part of a list is the range's first (slot 0) or, where its list begins, last (1)
       const int64_t slot = t_begin == 0 && t_end == n
@@ -617,8 +634,9 @@ __global__ void __launch_bounds__(128) window_decode_merge_kernel(const Args a) 
   if (n == 0) return;
   const int kvh = h / a.G, j = (h - kvh * a.G) / a.gc, hl = h - kvh * a.G - j * a.gc;
   const int64_t width = a.ws_plan[0];
+  const int open = (int)a.ws_plan[1];
   const int64_t first =  // place of the pair's first tile
-      a.ws_plan[1 + seq] * a.Hk + (int64_t)(kvh * a.hg + j) * places(n) + kOpen;
+      a.ws_plan[2 + seq] * a.Hk + (int64_t)(kvh * a.hg + j) * places(n, open) + open;
   const int64_t c0 = first / width;
   const int nsplit = (int)((first + n - 1) / width - c0) + 1;
   if (nsplit == 1) return;  // written whole
@@ -689,12 +707,12 @@ Plan make_plan(int64_t num_seqs, int Hq, int Hkv, int D, int64_t max_len, int wi
   const int64_t tiles = (keys + kKeys - 1) / kKeys + 2;
   const int64_t units = num_seqs * Hkv * p.hg, slots = (int64_t)kMaxPerSm * va_host::sm_count();
   if (tiles <= 2 * kMinRange || units >= 16 * slots) return p;
-  const int64_t most = units * ((tiles + kOpen + kMinRange - 1) / kMinRange);
+  const int64_t most = units * ((tiles + kOpenMost + kMinRange - 1) / kMinRange);
   p.most = (int)(most < slots ? most : slots);
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   p.o_ml = up((size_t)p.most * 2 * p.gc * D * 4);
   p.o_plan = p.o_ml + up((size_t)p.most * 2 * p.gc * 8);
-  p.total = p.o_plan + up((size_t)(num_seqs + 1) * 8);
+  p.total = p.o_plan + up((size_t)(num_seqs + 2) * 8);
   return p;
 }
 
