@@ -264,3 +264,29 @@ def test_one_token_chunks_agree_with_decode():
                                torch.tensor(c.lens, dtype=torch.int32).cuda(), scale=c.scale,
                                max_seq_len=1001, window=300, sink_tokens=4)
     c.check(out)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("bs,layout", [(16, "hnd"), (128, "nhd"), (24, "hnd")])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (4, 1, 96)])
+def test_cache_views(Hq, Hkv, D, bs, layout, q8):
+    """K and V interleaved in one tensor whose blocks, heads and rows have gaps."""
+    c = Case(Hq, Hkv, D, CHUNKS, bs=bs, layout=layout, q8=q8, window=200, sinks=5, seed=3)
+    nb, d1, d2, _ = c.kv[0].shape
+    big = torch.full((nb + 1, 2, d1 + 1, d2 + 1, D + 16), 127 if q8 else math.nan,
+                     dtype=c.kv[0].dtype)
+    for v in range(2):
+        big[:nb, v, :d1, :d2, :D] = c.kv[v]
+    big = big.cuda()
+    views = [big[:nb, v, :d1, :d2, :D] for v in range(2)]
+    if q8:
+        views = [x.view(torch.float8_e4m3fn) for x in views]
+    ks, vs = (None if e is None else e.cuda() for e in c.ex)
+    q = c.q.cuda()
+    out = torch.full_like(q, 7.0)
+    _ops().paged_window_prefill(
+        out, q, *views, c.table.cuda(), torch.tensor(c.start, dtype=torch.int32).cuda(),
+        torch.tensor(c.lens, dtype=torch.int32).cuda(), scale=c.scale, window=200,
+        sink_tokens=5, k_scale=ks, v_scale=vs, layout=layout)
+    assert _ops().check_device_errors() == 0
+    c.check(out)

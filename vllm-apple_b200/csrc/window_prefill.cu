@@ -5,7 +5,7 @@
 // One CTA takes a pair of 128-row tiles of one sequence and one kv head.  A row is a
 // (token, query head of the group) pair, so every staged key serves all heads of the
 // group and both tiles; the tiles' keys are the pair's key tiles of 128 (window.cuh), and
-// nothing outside the window and the sinks is read or multiplied.
+// no block without a key that some row sees is read, no tile without one multiplied.
 //   * warps 0-7: softmax, one thread per row (TMEM lane = row), warps 0-3 tile 0 and 4-7
 //     tile 1.  A row's 128 scores sit in the thread's registers (the other warps hand
 //     theirs over with setmaxnreg); P goes back over S as fp16 and feeds the second product
@@ -13,18 +13,33 @@
 //     more than 2^8, so O is rarely rescaled.
 //   * warp 8, one thread: issues tcgen05.mma for both tiles in turn -- PV_0(j-1), S_0(j),
 //     PV_1(j-1), S_1(j) -- so one tile's products run while the other is in its softmax.
-//   * warps 12-15: bring K and V key tiles into a ring of shared-memory slots in the
-//     128-byte-swizzled layout of the tensor core.  fp16 rows go there by 16-byte cp.async;
-//     e4m3 rows go to a raw buffer first and are turned into fp16 (exactly) from there.  Row addresses come from the block table once per key tile, so any block
-//     size and any strides work; keys that no row of the pair sees are zeros, unread.
+//   * fp16 cache: warp 9 brings K and V key tiles into a ring of shared-memory slots by TMA,
+//     one copy per block of the cache and 64 columns, in the 128-byte-swizzled layout of the
+//     tensor core.  Blocks that no row of the pair sees are copied from past the tensor's end,
+//     which gives zeros.  Block sizes that do not tile 128 keys (and cache layouts without a
+//     tensor map) take 16-byte cp.async from warps 12-15 instead, whose issue takes as long as
+//     a tile's products and softmax: four chunks of 512 under a window of 1024 (32 heads of 128
+//     over 8) 67.7 us by TMA, 76.6 by cp.async.
+//   * e4m3 cache: warps 12-19 copy rows by cp.async into a raw buffer two items ahead, and turn
+//     them into fp16 (exactly) in the slot.  TMA into a raw ring was 2 % faster on 8192 tokens
+//     and 2 % slower on short ones; four converting warps took 525 us instead of 502.
+//   Keys that no row of the pair sees are never part of a result: they are zeros, or their
+//   scores are masked for every row.
+// What bounds it: 8192 tokens under a window of 4096 over an e4m3 cache take 502 us (50 % of
+// the measured tensor peak for the visible products).  Alone, on the same grid,
+// the products take 368 us, the softmax 376, the conversion 319 and the barriers 223; the
+// products of one tile wait for its softmax, and the overlap of the two tiles hides some of
+// it.  Half-tile double buffering of S, P published in halves and polynomial powers were
+// slower; TMEM is full, so no third tile fits.
 // A key masked for one row but seen by another may hold an infinity or a NaN in V, and
 // 0 * inf would reach the masked row.  In key tiles that are masked in part (at most a
-// few per pair) the producers replace such values by 0, and rows that do see them get
+// few per pair) warps 12 on replace such values by 0, and rows that do see them get
 // them added at the end.
 // Scores, statistics and O are fp32; P is rounded to fp16.
 // Bounded waits: after a time-out every role runs its loop to the end without waiting or
 // issuing (so the roles still meet at their barriers), nothing is written and
 // VA_FLAG_WAIT_TIMEOUT is set.
+#include <cudaTypedefs.h>
 #include <limits.h>
 
 #include "prefill_tc.cuh"
@@ -35,21 +50,26 @@ namespace {
 constexpr int kRows = 128, kKeys = 128, kTiles = 2;
 constexpr int kSoftmax = kTiles * kRows;
 constexpr int kMmaWarp = kSoftmax / 32;
-constexpr int kProducers = 128;
-constexpr int kFirstProducer = kSoftmax + 128;  // warps 9-11 only lend their registers
-constexpr int kThreads = kFirstProducer + kProducers;
-// Registers: 512 threads launch with 128 each, the whole file; two warpgroups give up 64 a
-// thread and the softmax warpgroups take them: 2 x 128 x (192 + 64) = 512 x 128.
-constexpr int kRegsLaunch = 128, kRegsSoftmax = 192, kRegsOther = 64;
-static_assert(kThreads * kRegsLaunch == 65536 &&
-                  kSoftmax * kRegsSoftmax + (kThreads - kSoftmax) * kRegsOther == 65536,
-              "register shares");
-constexpr int kLag = 2;  // fp16 copies in flight behind the newest
+constexpr int kLoadWarp = kMmaWarp + 1;       // warps 10 and 11 only lend their registers
+constexpr int kFirstProducer = kSoftmax + 128;
+constexpr int kLag = 2;  // fp16 cp.async copies in flight behind the newest
+constexpr int kScrub = 4;  // barriers of V tiles that wait to be scrubbed (TMA)
 constexpr uint32_t kWaitLimit = 1u << 22;
 constexpr uint32_t kTmemO = kTiles * kKeys;  // TMEM: S of both tiles, then O of both
 
-template <int D, bool Q8>
+template <int D, bool Q8, bool TMA>
 struct Shape {
+  // An e4m3 cache takes eight warps to convert, an fp16 one four for what is left to do.
+  static constexpr int kProducers = Q8 ? 256 : 128;
+  static constexpr int kThreads = kFirstProducer + kProducers;
+  // Registers: the threads launch with kRegsLaunch each; the warpgroups past the softmax
+  // ones go down to kRegsOther and the softmax warpgroups take what they give up.
+  static constexpr int kRegsLaunch = Q8 ? 96 : 128, kRegsSoftmax = Q8 ? 168 : 192;
+  static constexpr int kRegsOther = Q8 ? 48 : 64;
+  static_assert(kThreads * kRegsLaunch <= 65536 &&
+                    kSoftmax * kRegsSoftmax + (kThreads - kSoftmax) * kRegsOther ==
+                        kThreads * kRegsLaunch,
+                "register shares");
   static constexpr int NB = (D + 63) / 64;            // 64-column blocks of a row
   static constexpr uint32_t kTileBytes = NB * 128 * 128;
   // fp16 key tiles of K or V; an e4m3 cache keeps two more as they come
@@ -57,13 +77,16 @@ struct Shape {
   static constexpr uint32_t kRawBytes = Q8 ? kKeys * D : 0;
   static constexpr uint32_t oSlot = kTiles * kTileBytes;
   static constexpr uint32_t oRaw = oSlot + kSlots * kTileBytes;
-  static constexpr uint32_t oInfo = oRaw + 2 * kRawBytes;  // int64 [128] row offsets
-  static constexpr uint32_t oExp = oInfo + 128 * 8;  // fp16 scales: K [128], V [2][128]
-  static constexpr uint32_t oBar = oExp + 3 * 128 * 2;
-  static constexpr uint32_t kBytes = oBar + 256 + 1024;  // + alignment slack
+  static constexpr uint32_t oInfo = oRaw + 2 * kRawBytes;  // int64 [128] row offsets (cp.async)
+  static constexpr uint32_t oExp = oInfo + (TMA ? 0 : 128 * 8);  // fp16 scales: K [128], V [2][128]
+  static constexpr uint32_t oBar = oExp + (Q8 ? 3 * 128 * 2 : 0);
+  static constexpr uint32_t kBars = 2 * kSlots + (TMA ? kScrub : 0) + 3 * kTiles + 2;
+  static constexpr uint32_t kBytes = oBar + kBars * 8 + 16 + 1024;  // + alignment slack
+  static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
 struct Args {
+  CUtensorMap mk, mv;  // boxes of one block of one head, or 128 tokens of it (TMA)
   __half *out;
   const __half *q;
   const uint8_t *kc, *vc, *ks, *vs;
@@ -118,7 +141,16 @@ VA_DEVINL void umma_commit(uint64_t *bar, uint32_t go) {
       : "memory");
 }
 
-VA_DEVINL void producer_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kProducers) : "memory"); }
+// 4-D tiled TMA load global -> shared, completion as tx bytes on `bar`.
+VA_DEVINL void tma_load_4d(void *dst, const CUtensorMap *map, int c0, int c1, int c2, int c3,
+                           uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(va::smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3),
+      "r"(va::smem_addr(bar))
+      : "memory");
+}
 
 // What a pair of tiles reads, in key tiles.
 struct Pair {
@@ -190,24 +222,27 @@ __noinline__ __device__ void add_not_finite(const Args &a, const int32_t *bt, in
   }
 }
 
-template <int D, bool Q8>
-__global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args a) {
-  using S = Shape<D, Q8>;
-  constexpr int NB = S::NB, kSlots = S::kSlots;
+template <int D, bool Q8, bool TMA>
+__global__ void __launch_bounds__(Shape<D, Q8, TMA>::kThreads, 1)
+    window_prefill_kernel(const __grid_constant__ Args a) {
+  using S = Shape<D, Q8, TMA>;
+  static_assert(!(Q8 && TMA), "e4m3 rows go through registers");
+  constexpr int NB = S::NB, kSlots = S::kSlots, kProducers = S::kProducers;
+  constexpr int kRegsSoftmax = S::kRegsSoftmax, kRegsOther = S::kRegsOther;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   // 128-byte swizzle atoms must sit on 1024-byte boundaries of the shared window
   unsigned char *smem = smem_raw + ((1024u - (va::smem_addr(smem_raw) & 1023u)) & 1023u);
   uint64_t *bar_full = reinterpret_cast<uint64_t *>(smem + S::oBar);  // [kSlots] tile landed
   uint64_t *bar_empty = bar_full + kSlots;   // [kSlots] MMAs that read the slot are done
-  uint64_t *bar_s = bar_empty + kSlots;      // [kTiles] S written
-  uint64_t *bar_p = bar_s + kTiles;          // [kTiles] P published (kRows arrivals)
+  uint64_t *bar_scrub = bar_empty + kSlots;  // [kScrub] a V tile to scrub landed (TMA)
+  uint64_t *bar_s = bar_scrub + (TMA ? kScrub : 0);  // [kTiles] S written
+  uint64_t *bar_p = bar_s + kTiles;          // [kTiles] P published (one arrival per warp)
   uint64_t *bar_o = bar_p + kTiles;          // [kTiles] PV done
   uint64_t *bar_q = bar_o + kTiles;          // Q staged
   uint64_t *bar_end = bar_q + 1;             // every MMA retired
   int *state = reinterpret_cast<int *>(bar_end + 1);
   int &s_dead = state[0], &s_bad = state[1], &s_poison = state[2];
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(state + 3);
-  static_assert((2 * kSlots + 3 * kTiles + 2) * 8 + 16 <= 256, "barrier space");
 
   va::pdl_enter();
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -256,15 +291,16 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
   if (tid == 0) {
     s_dead = s_bad = s_poison = 0;
     for (int i = 0; i < kSlots; ++i) {
-      va::mbar_init(&bar_full[i], kProducers);
+      va::mbar_init(&bar_full[i], TMA ? 1 : kProducers / 32);
       va::mbar_init(&bar_empty[i], 1);
     }
+    for (int i = 0; TMA && i < kScrub; ++i) va::mbar_init(&bar_scrub[i], 1);
     for (int h = 0; h < kTiles; ++h) {
       va::mbar_init(&bar_s[h], 1);
-      va::mbar_init(&bar_p[h], kRows);
+      va::mbar_init(&bar_p[h], kRows / 32);
       va::mbar_init(&bar_o[h], 1);
     }
-    va::mbar_init(bar_q, kSoftmax);
+    va::mbar_init(bar_q, kSoftmax / 32);
     va::mbar_init(bar_end, 1);
     va::fence_barrier_init();
   }
@@ -287,21 +323,38 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
     if (atomicExch(&s_dead, 1) == 0) va::raise_flag(a.err, VA_FLAG_WAIT_TIMEOUT);
   };
 
+  // A barrier counts warps: each thread's part is done, one lane arrives.
+  auto warp_arrive = [&](uint64_t *bar) {
+    __syncwarp();
+    if ((tid & 31) == 0) va::mbar_arrive(bar);
+  };
+  const int klo = win::run_start(pfirst, a.window);
+  // whether some row of the pair sees the key (a sink that only a later row's window has
+  // passed is inside the run [klo, plast])
+  auto seen = [&](int key) { return key <= plast && (key >= klo || key < a.sinks); };
+  auto slot_of = [&](int item) { return smem + S::oSlot + (item % kSlots) * S::kTileBytes; };
+  // whether the MMAs that read the item's slot before are done (without waiting), and a wait
+  auto is_empty = [&](int item) {
+    return item < kSlots || gone ||
+           va::mbar_try_wait(&bar_empty[item % kSlots], ((item / kSlots) - 1) & 1);
+  };
+  auto wait_empty = [&](int item) {
+    if (item >= kSlots) wait_bar(&bar_empty[item % kSlots], ((item / kSlots) - 1) & 1);
+  };
+
   if (tid >= kFirstProducer) {
     // =================== producers ===================
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    const int pt = tid - kFirstProducer;
+    const int pt = tid - kFirstProducer, kr = pt & (kKeys - 1);  // kr: its key row
     // element offset of each row of the key tile in the cache, | 1; 0: zeros
     int64_t *info = reinterpret_cast<int64_t *>(smem + S::oInfo);
-    uchar2 *exps = reinterpret_cast<uchar2 *>(smem + S::oExp);
-    const int klo = win::run_start(pfirst, a.window);
+    auto producer_sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(kProducers) : "memory"); };
     const int64_t head_off = kvh * a.s_head;
-    // block of key row pt of key tile j (-1: zeros)
+    // block of key row kr of key tile j (-1: zeros)
     auto block_of = [&](int j) -> int32_t {
       if (j >= nch) return -1;
-      const int key = win::tile_at(tl, j) * kKeys + pt;
-      // a sink that only a later row's window has passed is inside the run [klo, plast]
-      if (key > plast || (key < klo && key >= a.sinks)) return -1;
+      const int key = win::tile_at(tl, j) * kKeys + kr;
+      if (!seen(key)) return -1;
       const int32_t b = __ldg(bt + a.bs.div(key));
       if (b < 0 || b >= a.num_blocks) {
         va::raise_flag(a.err, VA_FLAG_BAD_BLOCK);
@@ -310,23 +363,14 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       }
       return b;
     };
-    auto off_of = [&](int j) { return a.bs.mod(win::tile_at(tl, j) * kKeys + pt); };
+    auto off_of = [&](int j) { return a.bs.mod(win::tile_at(tl, j) * kKeys + kr); };
     // (offsets are multiples of 8)
     auto row_of = [&](int32_t blk, int j) {
       return blk >= 0 ? (blk * a.s_block + head_off + off_of(j) * a.s_token) | 1 : int64_t(0);
     };
-    auto slot_of = [&](int item) { return smem + S::oSlot + (item % kSlots) * S::kTileBytes; };
-    // whether the MMAs that read the item's slot before are done (without waiting), and a wait
-    auto is_empty = [&](int item) {
-      return item < kSlots || gone ||
-             va::mbar_try_wait(&bar_empty[item % kSlots], ((item / kSlots) - 1) & 1);
-    };
-    auto wait_empty = [&](int item) {
-      if (item >= kSlots) wait_bar(&bar_empty[item % kSlots], ((item / kSlots) - 1) & 1);
-    };
     auto publish = [&](int item) {  // this thread's stores to the item's slot are visible
       va::fence_proxy_async_smem();
-      va::mbar_arrive(&bar_full[item % kSlots]);
+      warp_arrive(&bar_full[item % kSlots]);
     };
 
     if constexpr (!Q8) {
@@ -340,107 +384,127 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
         return P == 12 ? tc::sw128_off(piece_row(k), piece_col(k) * 8, kKeys)
                        : place0 + k * (kProducers / P) * 128;
       };
-      int32_t blk = block_of(0);
-      // an item's copies have landed -> scrub (V of a partly masked tile), publish
-      auto finish = [&](int item) {
-        if ((item & 1) && pr.partial(win::tile_at(tl, item >> 1))) {
-          unsigned char *sl = slot_of(item);
-          bool hit = false;
+      // V of a partly masked tile: no infinity or NaN stays
+      auto scrub = [&](int item) {
+        unsigned char *sl = slot_of(item);
+        const int key0 = win::tile_at(tl, item >> 1) * kKeys;
+        bool hit = false;
 #pragma unroll 4
-          for (int k = 0; k < P; ++k) {
-            uint4 *w = reinterpret_cast<uint4 *>(sl + place(k));
-            uint32_t x[4] = {w->x, w->y, w->z, w->w};
-            uint32_t h = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t bad = __vcmpgeu2(x[i] & 0x7fff7fffu, 0x7c007c00u);
-              h |= bad;
-              x[i] &= ~bad;
-            }
-            if (h) *w = make_uint4(x[0], x[1], x[2], x[3]);
-            hit = hit || h;
-          }
-          if (hit) *(volatile int *)&s_poison = 1;
-        }
-        publish(item);
-      };
-      int done = 0;  // items published
-      // Copies the item into its slot.  At most kLag items stay unpublished behind the newest
-      // one, and none while this thread waits for a slot.
-      auto copy = [&](int item) {
-        if (!is_empty(item)) {
-          if (item - done == 2) {
-            win::cp_async_wait<1>();
-            finish(done++);
-          }
-          if (item - done == 1) {
-            win::cp_async_wait<0>();
-            finish(done++);
-          }
-          wait_empty(item);
-        }
-        const __half *src = reinterpret_cast<const __half *>(item & 1 ? a.vc : a.kc);
-        const uint32_t sl = va::smem_addr(slot_of(item));
-#pragma unroll P == 12 ? 4 : P
         for (int k = 0; k < P; ++k) {
-          const int64_t e = info[piece_row(k)];
-          win::cp_async_zfill<16>(sl + place(k), src + (e & ~int64_t(7)) + piece_col(k) * 8, e & 1);
+          uint4 *w = reinterpret_cast<uint4 *>(sl + place(k));
+          uint32_t x[4] = {w->x, w->y, w->z, w->w};
+          uint32_t h = 0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t bad = __vcmpgeu2(x[i] & 0x7fff7fffu, 0x7c007c00u);
+            h |= bad;
+            x[i] &= ~bad;
+          }
+          if (h) {
+            *w = make_uint4(x[0], x[1], x[2], x[3]);
+            hit = hit || seen(key0 + piece_row(k));
+          }
         }
-        win::cp_async_commit();
-        if (item - done == kLag) {
-          win::cp_async_wait<kLag>();
-          finish(done++);
-        }
+        if (hit) *(volatile int *)&s_poison = 1;
       };
+      if constexpr (TMA) {
+        int n = 0;
 #pragma unroll 1
-      for (int j = 0; j < nch; ++j) {
-        producer_sync();  // everyone is done with the rows of the tile before
-        info[pt] = row_of(blk, j);
-        producer_sync();
-        blk = block_of(j + 1);
-        copy(2 * j);
-        copy(2 * j + 1);
-      }
-      win::cp_async_wait<0>();
-      while (done < 2 * nch) finish(done++);
-    } else {
-      // The codes of an item come by cp.async into one of two raw buffers, an item ahead;
-      // each thread turns the pieces it copied itself into fp16 in the item's slot.
-      constexpr int P = D / 16;  // 16-code pieces per row; each thread takes P of a tile
-      // piece k of this thread: row and column; rows a multiple of 8 apart unless P = 6, so
-      // that every address below is one base and a constant
-      auto piece_row = [&](int k) { return P == 6 ? (pt + k * kProducers) / 6 : pt / P + k * (kProducers / P); };
-      auto piece_col = [&](int k) { return P == 6 ? (pt + k * kProducers) % 6 : pt % P; };
-      unsigned char *raw = smem + S::oRaw + pt * 16;
-      __half *scale_k = reinterpret_cast<__half *>(smem + S::oExp), *scale_v = scale_k + kKeys;
-      int32_t blk0 = block_of(0), blk1 = block_of(1);
-      auto load_exps = [&](int32_t blk, int j) {
-        uchar2 e = make_uchar2(va::kQ8ExpBias, va::kQ8ExpBias);
-        if (blk >= 0) {
-          const int64_t at = blk * a.c_block + kvh * a.c_head + off_of(j) * a.c_token;
-          e.x = __ldg(a.ks + at);
-          e.y = __ldg(a.vs + at);
+        for (int j = 0; j < nch; ++j) {
+          if (!pr.partial(win::tile_at(tl, j))) continue;
+          wait_bar(&bar_scrub[n % kScrub], (n / kScrub) & 1);
+          scrub(2 * j + 1);
+          va::fence_proxy_async_smem();
+          producer_sync();
+          if (pt == 0) va::mbar_arrive(&bar_full[(2 * j + 1) % kSlots]);
+          ++n;
         }
-        return e;
+      } else {
+        int32_t blk = block_of(0);
+        // an item's copies have landed -> scrub, publish
+        auto finish = [&](int item) {
+          if ((item & 1) && pr.partial(win::tile_at(tl, item >> 1))) scrub(item);
+          publish(item);
+        };
+        int done = 0;  // items published
+        // Copies the item into its slot.  At most kLag items stay unpublished behind the newest
+        // one, and none while this thread waits for a slot.
+        auto copy = [&](int item) {
+          if (!is_empty(item)) {
+            if (item - done == 2) {
+              win::cp_async_wait<1>();
+              finish(done++);
+            }
+            if (item - done == 1) {
+              win::cp_async_wait<0>();
+              finish(done++);
+            }
+            wait_empty(item);
+          }
+          const __half *src = reinterpret_cast<const __half *>(item & 1 ? a.vc : a.kc);
+          const uint32_t sl = va::smem_addr(slot_of(item));
+#pragma unroll P == 12 ? 4 : P
+          for (int k = 0; k < P; ++k) {
+            const int64_t e = info[piece_row(k)];
+            win::cp_async_zfill<16>(sl + place(k), src + (e & ~int64_t(7)) + piece_col(k) * 8, e & 1);
+          }
+          win::cp_async_commit();
+          if (item - done == kLag) {
+            win::cp_async_wait<kLag>();
+            finish(done++);
+          }
+        };
+#pragma unroll 1
+        for (int j = 0; j < nch; ++j) {
+          producer_sync();  // everyone is done with the rows of the tile before
+          info[pt] = row_of(blk, j);
+          producer_sync();
+          blk = block_of(j + 1);
+          copy(2 * j);
+          copy(2 * j + 1);
+        }
+        win::cp_async_wait<0>();
+        while (done < 2 * nch) finish(done++);
+      }
+    } else {
+      // The codes of an item come by cp.async into one of two raw buffers, two items ahead;
+      // each thread turns the pieces it copied itself into fp16 in the item's slot.
+      constexpr int P = D / 16, N = P * kKeys / kProducers;  // 16-code pieces of a row, of a thread
+      // Piece k of this thread: row and column; rows a multiple of 8 apart unless P = 6, so
+      // that every address below is one base and a constant.  With P = 8 eight lanes take
+      // half of a row and the other half of the next: their codes lie in all banks, and so do
+      // their chunks 2c (and 2c + 1) in the swizzled slot, where the two halves of one row
+      // would share banks (546 -> 525 us for 8192 tokens under a window of 4096).
+      const int row0 = P == 8 ? (pt >> 4) * 2 + (pt >> 2 & 1) : pt / P;
+      const int col0 = P == 8 ? ((pt >> 1 ^ pt) & 4) + (pt & 3) : pt % P;
+      auto piece_row = [&](int k) { return P == 6 ? (pt + k * kProducers) / 6 : row0 + k * (kProducers / P); };
+      auto piece_col = [&](int k) { return P == 6 ? (pt + k * kProducers) % 6 : col0; };
+      unsigned char *raw = smem + S::oRaw + row0 * D + col0 * 16;  // + k * kProducers * 16
+      __half *scale_k = reinterpret_cast<__half *>(smem + S::oExp), *scale_v = scale_k + kKeys;
+      const bool is_k = pt < kKeys;  // whose exponents this thread brings
+      int32_t blk0 = block_of(0), blk1 = block_of(1);
+      auto load_exp = [&](int32_t blk, int j) -> uint32_t {
+        if (blk < 0) return va::kQ8ExpBias;
+        return __ldg((is_k ? a.ks : a.vs) + blk * a.c_block + kvh * a.c_head + off_of(j) * a.c_token);
       };
-      uchar2 e0 = load_exps(blk0, 0);
+      uint32_t e0 = load_exp(blk0, 0);
       // rows of key tile j and their scales for everyone; the next tile's exponents and block
       // are on their way
       auto announce = [&](int j) {
         producer_sync();  // K(j-1) is converted, V(j-1) on its way
-        info[pt] = row_of(blk0, j);
-        scale_k[pt] = __ushort_as_half((unsigned short)va::q8_scale_h2(e0.x));
-        scale_v[(j & 1) * kKeys + pt] = __ushort_as_half((unsigned short)va::q8_scale_h2(e0.y));
+        if (is_k) info[kr] = row_of(blk0, j);
+        (is_k ? scale_k : scale_v + (j & 1) * kKeys)[kr] =
+            __ushort_as_half((unsigned short)va::q8_scale_h2(e0));
         producer_sync();
         blk0 = blk1;
-        if (j + 1 < nch) e0 = load_exps(blk0, j + 1);
+        if (j + 1 < nch) e0 = load_exp(blk0, j + 1);
         blk1 = block_of(j + 2);
       };
       auto fetch = [&](int item) {
         const uint8_t *src = item & 1 ? a.vc : a.kc;
         const uint32_t to = va::smem_addr(raw + (item & 1) * S::kRawBytes);
 #pragma unroll
-        for (int k = 0; k < P; ++k) {
+        for (int k = 0; k < N; ++k) {
           const int64_t e = info[piece_row(k)];
           win::cp_async_zfill<16>(to + k * kProducers * 16, src + (e & ~int64_t(15)) + piece_col(k) * 16,
                                   e & 1);
@@ -451,20 +515,23 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
         const unsigned char *from = raw + (item & 1) * S::kRawBytes;
         unsigned char *sl = slot_of(item);
         const __half *scale = item & 1 ? scale_v + (item >> 1 & 1) * kKeys : scale_k;
-        const bool scrub = (item & 1) && pr.partial(win::tile_at(tl, item >> 1));
+        const int c = win::tile_at(tl, item >> 1);
+        const bool scrub = (item & 1) && pr.partial(c);
         uint32_t hit = 0;
 #pragma unroll
-        for (int k = 0; k < P; ++k) {
+        for (int k = 0; k < N; ++k) {
           const uint4 r = *reinterpret_cast<const uint4 *>(from + k * kProducers * 16);
           const uint32_t f = (uint32_t)__half_as_ushort(scale[piece_row(k)]) * 0x10001u;
           uint32_t w[4] = {r.x, r.y, r.z, r.w}, o[8];
           if (scrub) {
+            uint32_t any = 0;
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               const uint32_t bad = __vcmpeq4(w[x] & 0x7f7f7f7fu, 0x7f7f7f7fu);
-              hit |= bad;
+              any |= bad;
               w[x] &= ~bad;
             }
+            if (any && seen(c * kKeys + piece_row(k))) hit = 1;
           }
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
@@ -474,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
           }
           // 16-byte chunks 2c, 2c + 1 of the row; the first one's place differs by bit 4
           const uint32_t to = P == 6 ? tc::sw128_off(piece_row(k), piece_col(k) * 16, kKeys)
-                                     : tc::sw128_off(pt / P, pt % P * 16, kKeys) +
+                                     : tc::sw128_off(row0, col0 * 16, kKeys) +
                                            k * (kProducers / P) * 128;
           *reinterpret_cast<uint4 *>(sl + to) = make_uint4(o[0], o[1], o[2], o[3]);
           *reinterpret_cast<uint4 *>(sl + (to ^ 16)) = make_uint4(o[4], o[5], o[6], o[7]);
@@ -576,6 +643,68 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       if (!va::mbar_wait_bounded(bar_end, 0, kWaitLimit) && atomicExch(&s_dead, 1) == 0)
         va::raise_flag(a.err, VA_FLAG_WAIT_TIMEOUT);
       __syncwarp();
+    } else if (TMA && warp == kLoadWarp) {
+      // =================== TMA: one copy per block of a key tile ===================
+      const int lane = tid & 31;
+      const int rows = min((int)a.bs.d, kKeys), copies = kKeys / rows;  // lanes 0 .. copies - 1 copy
+      // block of the lane's copy for key tile j; num_blocks, past the tensor, gives zeros
+      auto block_of = [&](int j) -> int32_t {
+        const int key = win::tile_at(tl, j) * kKeys + lane * rows;
+        // some row sees one of its keys
+        if (lane >= copies || key > plast || (key + rows <= klo && key >= a.sinks))
+          return (int32_t)a.num_blocks;
+        const int32_t b = __ldg(bt + a.bs.div(key));
+        if (b >= 0 && b < a.num_blocks) return b;
+        va::raise_flag(a.err, VA_FLAG_BAD_BLOCK);
+        *(volatile int *)&s_bad = 1;
+        return (int32_t)a.num_blocks;
+      };
+      int items = 0, n = 0;  // issued; those that wait to be scrubbed
+      int32_t next = block_of(0);
+#pragma unroll 1
+      for (int j = 0; j < nch; ++j) {
+        const int c = win::tile_at(tl, j);
+        const int32_t blk = next;
+        const int off = a.bs.mod(c * kKeys + lane * rows);  // token of the block
+        if (j + 1 < nch) next = block_of(j + 1);
+        const bool part = pr.partial(c);
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const int item = 2 * j + v;
+          wait_empty(item);
+          if (__any_sync(0xffffffffu, gone)) {
+            gone = true;
+            continue;
+          }
+          uint64_t *bar = v && part ? &bar_scrub[n++ % kScrub] : &bar_full[item % kSlots];
+          if (lane == 0) va::mbar_arrive_expect_tx(bar, S::kTileBytes);
+          __syncwarp();
+          if (lane < copies) {
+            unsigned char *to = slot_of(item) + lane * rows * 128;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+              tma_load_4d(to + b * (kKeys * 128), v ? &a.mv : &a.mk, b * 64, off, kvh, blk, bar);
+          }
+          items = item + 1;
+        }
+      }
+      // After a time-out nobody else may wait for the copies in flight: they land (within a
+      // bounded wait) before the CTA's shared memory is given back.
+      if (__any_sync(0xffffffffu, gone) || dead()) {
+        bool landed = true;
+        auto land = [&](uint64_t *bar, uint32_t parity) {
+          landed = va::mbar_wait_bounded(bar, parity, kWaitLimit) && landed;
+        };
+        for (int i = 0, m = 0; i < items; ++i) {
+          if ((i & 1) && pr.partial(win::tile_at(tl, i >> 1))) {
+            if (m >= n - kScrub) land(&bar_scrub[m % kScrub], (m / kScrub) & 1);
+            ++m;
+          } else if (i >= items - kSlots) {
+            land(&bar_full[i % kSlots], (i / kSlots) & 1);
+          }
+        }
+        if (!landed) va::raise_flag(a.err, VA_FLAG_WAIT_TIMEOUT);
+      }
     }
   } else {
     // =================== Q, then softmax of tile h, one thread per row ===================
@@ -597,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       win::cp_async_commit();
       win::cp_async_wait<0>();
       va::fence_proxy_async_smem();
-      va::mbar_arrive(bar_q);
+      warp_arrive(bar_q);
     }
     const int tk = a.g.div(row), g = row - tk * a.G, ti = h * a.TQ + tk;
     const bool row_ok = tk < a.TQ && ti < nq && p0 + ti >= 0;
@@ -695,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
       l = l * alpha + ((y0 + y1) + (y2 + y3));
       tc::tmem_wait_st();
       tc::fence_before_sync();
-      va::mbar_arrive(&bar_p[h]);
+      warp_arrive(&bar_p[h]);
       ++n;
     }
     if (n > 0) {
@@ -742,26 +871,74 @@ __global__ void __launch_bounds__(kThreads, 1) window_prefill_kernel(const Args 
   }
 }
 
-template <int D, bool Q8>
+template <int D, bool Q8, bool TMA>
 int launch_t(const Args &a, unsigned grid, cudaStream_t st) {
+  using S = Shape<D, Q8, TMA>;
+  constexpr auto kernel = window_prefill_kernel<D, Q8, TMA>;
   static std::atomic<uint64_t> done{0};
   static std::atomic<int> regs{0};
-  if (!win::allow_smem(window_prefill_kernel<D, Q8>, (int)Shape<D, Q8>::kBytes, done))
-    return VA_ERR_LAUNCH;
+  if (!win::allow_smem(kernel, (int)S::kBytes, done)) return VA_ERR_LAUNCH;
   // the register shares only add up when the build gave every thread kRegsLaunch: with fewer
   // the softmax warps would wait for registers for good
   int r = regs.load(std::memory_order_relaxed);
   if (!r) {
     cudaFuncAttributes at;
-    if (cudaFuncGetAttributes(&at, window_prefill_kernel<D, Q8>) != cudaSuccess)
-      return VA_ERR_LAUNCH;
+    if (cudaFuncGetAttributes(&at, kernel) != cudaSuccess) return VA_ERR_LAUNCH;
     regs.store(r = at.numRegs, std::memory_order_relaxed);
   }
-  if (r != kRegsLaunch) return VA_ERR_LAUNCH;
-  if (va_host::launch_pdl_smem(window_prefill_kernel<D, Q8>, grid, kThreads, Shape<D, Q8>::kBytes, st,
-                               a))
-    return VA_ERR_LAUNCH;
+  if (r != S::kRegsLaunch) return VA_ERR_LAUNCH;
+  if (va_host::launch_pdl_smem(kernel, grid, S::kThreads, S::kBytes, st, a)) return VA_ERR_LAUNCH;
   return va_host::launch_status();
+}
+
+using Encode = PFN_cuTensorMapEncodeTiled_v12000;
+Encode encoder() {
+  static const Encode fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void *f = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<Encode>(f);
+  }();
+  return fn;
+}
+
+// Tensor maps over (head dim, token of the block, kv head, block) of the fp16 caches: a box is
+// 64 columns of one block of one head, or of 128 tokens of a longer block, and lands in the
+// tensor core's 128-byte swizzle (columns past the head size are zeros).  Blocks that do not
+// tile 128 keys in pieces of at least 8 rows (one swizzle atom), and layouts that the encoder
+// does not take, leave the copies to cp.async.
+bool encode_maps(Args &a, int D) {
+  const int bs = (int)a.bs.d, rows = bs < kKeys ? bs : kKeys;
+  if (bs < 8 || (bs < kKeys ? kKeys % bs : bs % kKeys) || a.num_blocks == 0 ||
+      a.num_blocks >= INT32_MAX)
+    return false;
+  const Encode enc = encoder();
+  if (!enc) return false;
+  const int64_t extent[3] = {bs, a.Hkv, a.num_blocks}, stride[3] = {a.s_token, a.s_head, a.s_block};
+  cuuint64_t dims[4] = {(cuuint64_t)D}, strides[3];
+  for (int i = 0; i < 3; ++i) {
+    if (extent[i] > 1 && (stride[i] <= 0 || stride[i] >= int64_t(1) << 38)) return false;
+    dims[i + 1] = (cuuint64_t)extent[i];
+    strides[i] = (cuuint64_t)(extent[i] > 1 ? stride[i] : D) * 2;  // of one element: never used
+  }
+  const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, one[4] = {1, 1, 1, 1};
+  for (int v = 0; v < 2; ++v)
+    if (enc(v ? &a.mv : &a.mk, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+            const_cast<uint8_t *>(v ? a.vc : a.kc), dims, strides, box, one,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            D > 64 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return false;
+  return true;
+}
+
+template <int D>
+int launch_d(Args &a, bool q8, unsigned grid, cudaStream_t st) {
+  if (q8) return launch_t<D, true, false>(a, grid, st);
+  return encode_maps(a, D) ? launch_t<D, false, true>(a, grid, st)
+                           : launch_t<D, false, false>(a, grid, st);
 }
 
 }  // namespace
@@ -830,15 +1007,12 @@ extern "C" int va_window_prefill(void *out, const void *q, const void *k_cache,
   if (pairs * num_kv_heads > INT32_MAX) return VA_ERR_UNSUPPORTED;
   const unsigned grid = (unsigned)(pairs * num_kv_heads);
   auto st = static_cast<cudaStream_t>(stream);
-  switch (head_size + (kv_e4m3 ? 1 : 0)) {
-    case 32: return launch_t<32, false>(a, grid, st);
-    case 33: return launch_t<32, true>(a, grid, st);
-    case 64: return launch_t<64, false>(a, grid, st);
-    case 65: return launch_t<64, true>(a, grid, st);
-    case 96: return launch_t<96, false>(a, grid, st);
-    case 97: return launch_t<96, true>(a, grid, st);
-    case 128: return launch_t<128, false>(a, grid, st);
-    case 129: return launch_t<128, true>(a, grid, st);
+  const bool q8 = kv_e4m3 != 0;
+  switch (head_size) {
+    case 32: return launch_d<32>(a, q8, grid, st);
+    case 64: return launch_d<64>(a, q8, grid, st);
+    case 96: return launch_d<96>(a, q8, grid, st);
+    case 128: return launch_d<128>(a, q8, grid, st);
   }
   return VA_ERR_UNSUPPORTED;
 }
