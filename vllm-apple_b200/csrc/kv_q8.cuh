@@ -58,13 +58,6 @@ VA_DEVINL uint32_t q8_encode4(uint32_t a, uint32_t b, uint32_t inv) {
   return r;
 }
 
-// Two e4m3 codes (the low 16 bits of `c`) as fp16, low byte -> low half.
-VA_DEVINL uint32_t q8_decode2(uint32_t c) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)c));
-  return r;
-}
-
 // Four e4m3 codes as two fp16 pairs.
 VA_DEVINL void q8_decode4(uint32_t c, uint32_t &lo, uint32_t &hi) {
   asm("{\n\t.reg .b16 l, h;\n\t"
