@@ -210,7 +210,7 @@ VA_DEVINL Range find_range(const Args &a) {
   return r;
 }
 
-// The new K (threads 0..15) and V (threads 16..31) row of one kv head into the cache.
+// The new K (lanes 0..15) and V (lanes 16..31) row of one kv head into the cache.
 template <int D, bool Q8>
 VA_DEVINL void write_new_row(const Args &a, int seq, int kvh, int64_t blk, int off) {
   const int sub = threadIdx.x & 15;
@@ -242,7 +242,7 @@ VA_DEVINL void write_new_row(const Args &a, int seq, int kvh, int64_t blk, int o
 // One part: tiles [t_begin, t_end) of one head group of one sequence.  `slot` >= 0: not
 // the whole list of its tiles, so the result goes to that slot of the workspace.
 template <int D, bool Q8, int NT>
-VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int &s_bad, int seq, int hk, int L,
+VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int *s_bad, int seq, int hk, int L,
                            const win::Tiles &tl, int t_begin, int t_end, int64_t slot) {
   using S = Shape<D, Q8>;
   const int kvh = hk / a.hg, head0 = kvh * a.G + (hk - kvh * a.hg) * a.gc;
@@ -250,16 +250,6 @@ VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int &s_bad, int s
   const int lo = win::run_start(L - 1, a.window);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int32_t *bt = a.bt + seq * a.max_blocks;
-  if (threadIdx.x == 0) s_bad = 0;
-
-  // The part that reads the newest key writes it first, then reads it back with the rest.
-  if (a.nk && t_end == tl.count) {
-    const int page = a.bs.div(L - 1);
-    const int32_t blk = __ldg(bt + page);
-    if (threadIdx.x < 32 && blk >= 0 && blk < a.num_blocks)
-      write_new_row<D, Q8>(a, seq, kvh, blk, L - 1 - page * (int)a.bs.d);
-  }
-
   // Q^T fragments: columns = heads, rows in the order of the K fragments below
   uint32_t qf[NT][D / 16][2];
 #pragma unroll
@@ -274,7 +264,6 @@ VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int &s_bad, int s
       qf[n][ks][0] = w.x;
       qf[n][ks][1] = w.y;
     }
-  __syncthreads();
 
   // ---- copy pipeline: tile i of this warp is key tile t_begin + warp + i * kNW ----
   constexpr int KT = S::KT, R = S::kStages;
@@ -370,8 +359,21 @@ VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int &s_bad, int s
     }
     win::cp_async_commit();
   };
+  // The warp that reads the newest key (its last tile) writes it before, and reads it back
+  // with the rest; its first copies are on their way by then where they do not hold it.
+  constexpr int kAhead = R / KT - 1;  // passes
+  const bool writes = a.nk && t_end == tl.count && warp == (t_end - 1 - t_begin) % kNW;
+  auto write = [&]() {
+    const int page = a.bs.div(L - 1);
+    const int32_t to = __ldg(bt + page);
+    if (to >= 0 && to < a.num_blocks)
+      write_new_row<D, Q8>(a, seq, kvh, to, L - 1 - page * (int)a.bs.d);
+    __syncwarp();  // for the lanes that copy it
+  };
+  if (writes && npass <= kAhead) write();
 #pragma unroll
-  for (int p = 0; p < R / KT - 1; ++p) copy_pass(p);
+  for (int p = 0; p < kAhead; ++p) copy_pass(p);
+  if (writes && npass > kAhead) write();
 
   float m[NT][2], l[NT][2], o[NT][D / 16][4];
 #pragma unroll
@@ -385,8 +387,8 @@ VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int &s_bad, int s
   int rslot = 0;
 #pragma unroll 1
   for (int i = 0; i < npass; ++i) {
-    copy_pass(i + R / KT - 1);
-    win::cp_async_wait<R / KT - 1>();
+    copy_pass(i + kAhead);
+    win::cp_async_wait<kAhead>();
     __syncwarp();  // other lanes' copies and exponents
     const unsigned char *st0 = ring + rslot * S::kStage;
     // ---- S^T = K Q^T ----
@@ -532,7 +534,8 @@ VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int &s_bad, int s
       l[n][0] += __shfl_xor_sync(0xffffffffu, l[n][0], w);
       l[n][1] += __shfl_xor_sync(0xffffffffu, l[n][1], w);
     }
-  if (bad) s_bad = 1;
+  bad = __any_sync(0xffffffffu, bad);
+  if (lane == 0) s_bad[warp] = bad;
   __syncthreads();  // the ring is free: the warps' results go there
 
   // value e of lane g lies at e * 8 + g of its head's row: stores hit every bank once
@@ -557,7 +560,9 @@ VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int &s_bad, int s
     }
   }
   __syncthreads();
-  const bool skip = s_bad != 0;
+  bool skip = false;
+#pragma unroll
+  for (int w = 0; w < kNW; ++w) skip = skip || s_bad[w] != 0;
   if (skip && threadIdx.x == 0) va::raise_flag(a.err, VA_FLAG_BAD_BLOCK);
   for (int i = threadIdx.x; i < nheads * D; i += kNW * 32) {
     const int h = i / D, d = i - h * D;
@@ -589,7 +594,7 @@ VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int &s_bad, int s
 template <int D, bool Q8, int NT>
 __global__ void __launch_bounds__(kNW * 32) window_decode_kernel(const Args a) {
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int s_bad;
+  __shared__ int s_bad[kNW];
   va::pdl_enter();
   if (a.ranges == 0) {  // a CTA per (sequence, head group)
     const int seq = blockIdx.x / a.Hk, hk = blockIdx.x - seq * a.Hk;
