@@ -28,10 +28,11 @@
 //     kernel, launched as a programmatic dependent, merges in list order.
 //   * Keys that the query does not see are zero-filled, never read: what lies in the
 //     cache behind a sequence, before its window or in a freed block does not matter.
-// Measured (32 heads of 128 over 8): 128 sequences under a window of 1024, fp16, 97 us (5.5
-// TB/s); 128 ragged e4m3 contexts of up to 8192 tokens 206-216 us (5.4 TB/s), one of 131000
+// Measured (32 heads of 128 over 8): 128 sequences under a window of 1024, fp16, 95 us (5.6
+// TB/s); 128 ragged e4m3 contexts of up to 8192 tokens 211-218 us (5.2 TB/s), one of 131000
 // 60 us (4.5 TB/s).  A stream of tiles per warp instead of per CTA took 273 and 74 us for the
-// last two, two waves of ranges more than one.  Small calls (4 sequences under a window of
+// last two, two waves of ranges more than one.  The copies
+// alone, without products, take 210 and 53 us of them, the products alone 132 and 42.  Small calls (4 sequences under a window of
 // 128, 14 heads of 64 over 2: 4.7 us) are two launches and one chain of copies and merges.
 #include "window.cuh"
 
