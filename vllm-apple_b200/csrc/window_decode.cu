@@ -30,10 +30,11 @@
 //     cache behind a sequence, before its window or in a freed block does not matter.
 // Measured (32 heads of 128 over 8): 128 sequences under a window of 1024, fp16, 95 us (5.6
 // TB/s); 128 ragged e4m3 contexts of up to 8192 tokens 211-218 us (5.2 TB/s), one of 131000
-// 60 us (4.5 TB/s).  A stream of tiles per warp instead of per CTA took 273 and 74 us for the
-// last two, two waves of ranges more than one.  The copies
-// alone, without products, take 210 and 53 us of them, the products alone 132 and 42.  Small calls (4 sequences under a window of
-// 128, 14 heads of 64 over 2: 4.7 us) are two launches and one chain of copies and merges.
+// 60 us (4.5 TB/s).  The copies alone, without products, take 210 and 53 us of the last two,
+// the products alone 132 and 42.  A stream of tiles per warp instead of per CTA took 273 and
+// 74 us, two or eight warps per CTA 269 and 251 us for the contexts, two waves of ranges more
+// than one.  Small calls (4 sequences under a window of 128, 14 heads of 64 over 2: 4.6 us)
+// are launches and one chain of dependent loads.
 #include "window.cuh"
 
 namespace {

@@ -377,7 +377,9 @@ __global__ void __launch_bounds__(Shape<D, Q8, TMA>::kThreads, 1)
       constexpr int P = D / 8;  // 16-byte pieces per row; each thread copies P of a tile
       // piece k of this thread: row, column and place in a slot; rows a multiple of 8 apart
       // unless P = 12, so that the places are one base and a constant
-      auto piece_row = [&](int k) { return P == 12 ? (pt + k * kProducers) / 12 : pt / P + k * (kProducers / P); };
+      auto piece_row = [&](int k) {
+        return P == 12 ? (pt + k * kProducers) / 12 : pt / P + k * (kProducers / P);
+      };
       auto piece_col = [&](int k) { return P == 12 ? (pt + k * kProducers) % 12 : pt % P; };
       const uint32_t place0 = tc::sw128_off(pt / P, pt % P * 8, kKeys);
       auto place = [&](int k) {
@@ -477,7 +479,9 @@ __global__ void __launch_bounds__(Shape<D, Q8, TMA>::kThreads, 1)
       // would share banks (546 -> 525 us for 8192 tokens under a window of 4096).
       const int row0 = P == 8 ? (pt >> 4) * 2 + (pt >> 2 & 1) : pt / P;
       const int col0 = P == 8 ? ((pt >> 1 ^ pt) & 4) + (pt & 3) : pt % P;
-      auto piece_row = [&](int k) { return P == 6 ? (pt + k * kProducers) / 6 : row0 + k * (kProducers / P); };
+      auto piece_row = [&](int k) {
+        return P == 6 ? (pt + k * kProducers) / 6 : row0 + k * (kProducers / P);
+      };
       auto piece_col = [&](int k) { return P == 6 ? (pt + k * kProducers) % 6 : col0; };
       unsigned char *raw = smem + S::oRaw + row0 * D + col0 * 16;  // + k * kProducers * 16
       __half *scale_k = reinterpret_cast<__half *>(smem + S::oExp), *scale_v = scale_k + kKeys;
