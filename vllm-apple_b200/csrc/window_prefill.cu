@@ -22,15 +22,15 @@
 //     over 8) 67.7 us by TMA, 76.6 by cp.async.
 //   * e4m3 cache: warps 12-19 copy rows by cp.async into a raw buffer two items ahead, and turn
 //     them into fp16 (exactly) in the slot.  TMA into a raw ring was 2 % faster on 8192 tokens
-//     and 2 % slower on short ones; four converting warps took 525 us instead of 502.
+//     and 2 % slower on short ones; four converting warps took 525 us where eight took 502.
 //   Keys that no row of the pair sees are never part of a result: they are zeros, or their
 //   scores are masked for every row.
-// What bounds it: 8192 tokens under a window of 4096 over an e4m3 cache take 502 us (50 % of
-// the measured tensor peak for the visible products).  Alone, on the same grid,
-// the products take 368 us, the softmax 376, the conversion 319 and the barriers 223; the
-// products of one tile wait for its softmax, and the overlap of the two tiles hides some of
-// it.  Half-tile double buffering of S, P published in halves and polynomial powers were
-// slower; TMEM is full, so no third tile fits.
+// What bounds it: 8192 tokens under a window of 4096 over an e4m3 cache take 480 us (52 % of
+// the measured tensor peak for the visible products).  Alone, on the same grid (of a build
+// that took 491), the products take 368 us, the softmax 376, the conversion 319 and the
+// barriers 223; the products of one tile wait for its softmax, and the overlap of the two
+// tiles hides some of it.  Half-tile double buffering of S, P published in halves and
+// polynomial powers were slower; TMEM is full, so no third tile fits.
 // A key masked for one row but seen by another may hold an infinity or a NaN in V, and
 // 0 * inf would reach the masked row.  In key tiles that are masked in part (at most a
 // few per pair) warps 12 on replace such values by 0, and rows that do see them get
@@ -63,11 +63,13 @@ struct Shape {
   static constexpr int kProducers = Q8 ? 256 : 128;
   static constexpr int kThreads = kFirstProducer + kProducers;
   // Registers: the threads launch with kRegsLaunch each; the warpgroups past the softmax
-  // ones go down to kRegsOther and the softmax warpgroups take what they give up.
-  static constexpr int kRegsLaunch = Q8 ? 96 : 128, kRegsSoftmax = Q8 ? 168 : 192;
-  static constexpr int kRegsOther = Q8 ? 48 : 64;
+  // ones go down to kRegsOther and the softmax warpgroups take what they give up.  e4m3, 8192
+  // tokens: 502 us with 168 and 48, 480 with 176 and 40, 510 with 184 and 32; fp16 does not
+  // change from 184 to 208.
+  static constexpr int kRegsLaunch = Q8 ? 96 : 128, kRegsSoftmax = Q8 ? 176 : 192;
+  static constexpr int kRegsOther = Q8 ? 40 : 64;
   static_assert(kThreads * kRegsLaunch <= 65536 &&
-                    kSoftmax * kRegsSoftmax + (kThreads - kSoftmax) * kRegsOther ==
+                    kSoftmax * kRegsSoftmax + (kThreads - kSoftmax) * kRegsOther <=
                         kThreads * kRegsLaunch,
                 "register shares");
   static constexpr int NB = (D + 63) / 64;            // 64-column blocks of a row
