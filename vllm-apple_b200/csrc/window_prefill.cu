@@ -9,8 +9,9 @@
 //   * warps 0-7: softmax, one thread per row (TMEM lane = row), warps 0-3 tile 0 and 4-7
 //     tile 1.  A row's 128 scores sit in the thread's registers (the other warps hand
 //     theirs over with setmaxnreg); P goes back over S as fp16 and feeds the second product
-//     from TMEM.  The maximum a row's powers are taken against only moves when it grows by
-//     more than 2^8, so O is rarely rescaled.
+//     from TMEM.  The maximum a row's powers are taken against only moves when a power
+//     would pass 2^12 (fp16 ends at 2^16), so O is rarely rescaled: 494 us (of 8192 tokens,
+//     below) with 2^6, 480 with 2^8, 476 from 2^10 on.
 //   * warp 8, one thread: issues tcgen05.mma for both tiles in turn -- PV_0(j-1), S_0(j),
 //     PV_1(j-1), S_1(j) -- so one tile's products run while the other is in its softmax.
 //   * fp16 cache: warp 9 brings K and V key tiles into a ring of shared-memory slots by TMA,
@@ -25,7 +26,7 @@
 //     and 2 % slower on short ones; four converting warps took 525 us where eight took 502.
 //   Keys that no row of the pair sees are never part of a result: they are zeros, or their
 //   scores are masked for every row.
-// What bounds it: 8192 tokens under a window of 4096 over an e4m3 cache take 480 us (52 % of
+// What bounds it: 8192 tokens under a window of 4096 over an e4m3 cache take 476 us (53 % of
 // the measured tensor peak for the visible products).  Alone, on the same grid (of a build
 // that took 491), the products take 368 us, the softmax 376, the conversion 319 and the
 // barriers 223; the products of one tile wait for its softmax, and the overlap of the two
@@ -787,7 +788,7 @@ __global__ void __launch_bounds__(Shape<D, Q8, TMA>::kThreads, 1)
       mx[1] = tc::fmax3(mx[1], p[kKeys - 2], p[kKeys - 1]);
       float rmax = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       rmax *= sc;  // the scale is positive
-      const float mn = (m == -INFINITY || rmax > m + 8.f) ? fmaxf(m, rmax) : m;
+      const float mn = (m == -INFINITY || rmax > m + 12.f) ? fmaxf(m, rmax) : m;
       const bool none = mn == -INFINITY;  // no visible key so far
       const float alpha = (none || mn == m) ? 1.f : va::fast_exp2(m - mn);
       const float nm = none ? 0.f : -mn;
