@@ -35,12 +35,18 @@
 // 74 us, two or eight warps per CTA 269 and 251 us for the contexts, two waves of ranges more
 // than one.  Small calls (4 sequences under a window of 128, 14 heads of 64 over 2: 4.6 us)
 // are launches and one chain of dependent loads.
+#include <float.h>
+
 #include "window.cuh"
 
 namespace {
 
 constexpr int kNW = 4;  // warps per CTA
 constexpr int kKeys = 16;
+// Where a maximum begins.  Scores that are -inf (masked keys, an infinity in a K row) do not
+// move it, and their powers are 0; from -inf they would be the NaN of -inf - -inf, which other
+// keys' results could not take back.  No finite score lies below.
+constexpr float kLowest = -FLT_MAX;
 
 template <int D, bool Q8>
 struct Shape {
@@ -380,7 +386,7 @@ VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int *s_bad, int s
   float m[NT][2], l[NT][2], o[NT][D / 16][4];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
-    m[n][0] = m[n][1] = -INFINITY;
+    m[n][0] = m[n][1] = kLowest;
     l[n][0] = l[n][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.f;
@@ -470,7 +476,6 @@ VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int *s_bad, int s
           o[n][k][3] *= f1;
         }
       }
-      // every pass holds a visible key, so m is finite unless a score is not
 #pragma unroll
       for (int u = 0; u < KT; ++u) {
         const float x0 = va::fast_exp2(s[u][n][0] - m0), x1 = va::fast_exp2(s[u][n][1] - m1);
@@ -575,8 +580,8 @@ VA_DEVINL void decode_part(const Args &a, unsigned char *smem, int *s_bad, int s
     float A = 0.f, Ls = 0.f;
 #pragma unroll
     for (int w = 0; w < kNW; ++w) {
-      // a warp without tiles has m = -inf and adds nothing
-      const float f = sm[w * NH + h] == -INFINITY ? 0.f : va::fast_exp2(sm[w * NH + h] - M);
+      // (a warp without tiles adds zeros)
+      const float f = va::fast_exp2(sm[w * NH + h] - M);
       A += so[(w * NH + h) * HS + at] * f;
       Ls += sl[w * NH + h] * f;
     }
@@ -656,7 +661,7 @@ __global__ void __launch_bounds__(128) window_decode_merge_kernel(const Args a) 
   auto part = [&](int s) -> int64_t { return (2 * (c0 + s) + (s == 0 ? 1 : 0)) * a.gc + hl; };
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // every warp finds the common maximum, 32 ranges at a time
-  float M = -INFINITY;
+  float M = kLowest;
   bool skip = false;
   for (int s = lane; s < nsplit; s += 32) {
     const float2 v = a.ws_ml[part(s)];
@@ -673,7 +678,7 @@ __global__ void __launch_bounds__(128) window_decode_merge_kernel(const Args a) 
   for (int s = warp; s < nsplit; s += 4) {
     const int64_t p = part(s);
     const float2 v = a.ws_ml[p];
-    const float f = v.x == -INFINITY ? 0.f : va::fast_exp2(v.x - M);
+    const float f = va::fast_exp2(v.x - M);
     Ls = fmaf(v.y, f, Ls);
 #pragma unroll
     for (int e = 0; e < E; ++e)
