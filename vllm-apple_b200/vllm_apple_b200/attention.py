@@ -74,6 +74,12 @@ except Exception:  # pragma: no cover - exercised only where vLLM is absent
 
     split_decodes_and_prefills = None
 
+try:  # cache specs whose manager frees the blocks that a window has passed
+    from vllm.v1.kv_cache_interface import ChunkedLocalAttentionSpec, SlidingWindowSpec
+    _FREEING_SPECS: tuple = (SlidingWindowSpec, ChunkedLocalAttentionSpec)
+except Exception:  # pragma: no cover - exercised only where vLLM is absent
+    _FREEING_SPECS = ()
+
 
 class MetalAttentionBackend(AttentionBackend):
     """Paged attention with the fused KV write on B200 (backend name kept)."""
@@ -195,6 +201,7 @@ class MetalAttentionMetadataBuilder(AttentionMetadataBuilder[MetalAttentionMetad
         self.head_dim = kv_cache_spec.head_size
         self.dtype = vllm_config.model_config.dtype
         self.block_size = vllm_config.cache_config.block_size
+        _refuse_freed_sinks(kv_cache_spec, layer_names, vllm_config)
 
     def build(self, common_prefix_len: int, common_attn_metadata, fast_build: bool = False
               ) -> MetalAttentionMetadata:
@@ -217,6 +224,23 @@ class MetalAttentionMetadataBuilder(AttentionMetadataBuilder[MetalAttentionMetad
         if scpu is not None:
             md._seq_lens_cpu = scpu.tolist()
         return md
+
+
+def _refuse_freed_sinks(kv_cache_spec, layer_names, vllm_config) -> None:
+    """A layer with sink tokens reads its sequences' first blocks at every step.  A cache
+    manager that frees the blocks behind the window puts the (valid) null block in their
+    place, which no check on the device can tell from a sink's."""
+    if not isinstance(kv_cache_spec, _FREEING_SPECS):
+        return
+    config = getattr(vllm_config, "compilation_config", None)
+    layers = getattr(config, "static_forward_context", None) or {}
+    for name in layer_names:
+        sinks = getattr(getattr(layers.get(name), "impl", None), "window_sink_tokens", None)
+        if sinks:
+            raise ValueError(
+                f"{name} keeps its first {sinks} tokens visible (window_sink_tokens), but its "
+                f"KV cache ({type(kv_cache_spec).__name__}) frees them once the window has "
+                "passed: give the layer a full-attention cache, or window_sink_tokens=0")
 
 
 def _i32(t: torch.Tensor) -> torch.Tensor:
@@ -261,7 +285,9 @@ class MetalAttentionImpl(AttentionImpl):
         self.sinks = sinks
         # A layer that asks for it (vLLM passes extra keyword arguments of a layer on) has its
         # sliding window applied, with that many first tokens kept visible (0: none).  Without
-        # it the window is carried and not applied, as in the reference's kernels.
+        # it the window is carried and not applied, as in the reference's kernels.  A layer with
+        # sink tokens needs a KV cache that keeps a sequence's first ceil(S / block_size) blocks
+        # (full attention's does); the metadata builder refuses one that frees them.
         self.window_sink_tokens = window_sink_tokens
         self._window = 0
         if window_sink_tokens is not None:
