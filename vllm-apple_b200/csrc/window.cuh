@@ -35,8 +35,10 @@ VA_DEVINL Tiles key_tiles(int first, int last, int window, int sinks, int size) 
 VA_DEVINL int tile_at(const Tiles &t, int i) { return i < t.sinks ? i : t.start + i - t.sinks; }
 
 // Division of keys (0 <= n < 2^31) by a block size that is only known at launch, as one
-// multiplication: m = ceil(2^(32 + sh) / d) with 2^sh the power of two that is not below
-// d leaves a remainder too small to matter for n < 2^31.
+// multiplication by m = ceil(2^(32 + sh) / d), where 2^sh < d <= 2^(sh + 1).
+//   * 2^sh < d, so m is below 2^32 and fits its field.
+//   * m d - 2^(32 + sh) < d, so n m / 2^(32 + sh) exceeds n / d by less than n / 2^(32 + sh).
+//     That is less than 1 / d, since n d < 2^31 2^(sh + 1): the floor is n / d's.
 struct FastDiv {
   uint32_t d, m, sh;
   VA_DEVINL int div(int n) const {
@@ -49,8 +51,7 @@ inline FastDiv fast_div(int d) {
   FastDiv f{};
   f.d = (uint32_t)d;
   if (d > 1) {
-    // sh = ceil(log2 d) - 1 keeps m in 32 bits
-    uint32_t sh = 0;
+    uint32_t sh = 0;  // ceil(log2 d) - 1
     while ((uint64_t(2) << sh) < (uint64_t)d) ++sh;
     f.sh = sh;
     f.m = (uint32_t)(((uint64_t(1) << (32 + sh)) + d - 1) / d);
