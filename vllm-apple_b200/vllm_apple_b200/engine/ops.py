@@ -331,15 +331,15 @@ class WindowedAttentionOp:
         lib = _lib.load()
         D, Hq, Hkv = self.head_size, self.num_query_heads, self.num_kv_heads
         k, v, ks, vs, e4m3, blocks = self._cache(kb, vb, ksb, vsb)
-        nbytes = lib.va_window_decode_workspace_size(num_seqs, Hq, Hkv, D, max_seq_len,
-                                                     self.window, self.sink_tokens)
+        visible = _ops.visibility(self.window, self.sink_tokens)
+        nbytes = lib.va_window_decode_workspace_size(num_seqs, Hq, Hkv, D, max_seq_len, *visible)
         ws = _ops.call_workspace(_dev(step_ctx), "window_decode", nbytes, step_ctx.stream)
         _lib.check(lib.va_window_decode(
             resolve(ob, oo)[0], resolve(qb, qo)[0], k, v, ks, vs, e4m3, resolve(btb)[0],
             resolve(slb)[0], nk, nv, num_seqs, Hq, Hkv, D, self.block_size, max_blocks,
-            max_seq_len, blocks, float(self.scale), self.window, self.sink_tokens,
-            *self._cache_strides, *self._scale_strides, *self._row_strides, *self._row_strides,
-            Hkv * D, D, None if ws is None else ws.data_ptr(), nbytes, _err(step_ctx),
+            max_seq_len, blocks, float(self.scale), *visible, *self._cache_strides,
+            *self._scale_strides, *self._row_strides, *self._row_strides, Hkv * D, D,
+            None if ws is None else ws.data_ptr(), nbytes, _err(step_ctx),
             step_ctx.stream_handle), "va_window_decode")
         step_ctx.note_dispatch(2 if nbytes else 1)
 
@@ -359,9 +359,9 @@ class WindowedAttentionOp:
             ks, vs, e4m3, resolve(block_table_buffer)[0], resolve(query_start_loc_buffer)[0],
             resolve(seq_lens_buffer)[0], num_tokens, num_seqs, self.num_query_heads,
             self.num_kv_heads, self.head_size, self.block_size, max_blocks_per_seq, blocks,
-            float(self.scale), self.window, self.sink_tokens, *self._cache_strides,
-            *self._scale_strides, *self._row_strides, *self._row_strides, _err(step_ctx),
-            step_ctx.stream_handle), "va_window_prefill")
+            float(self.scale), *_ops.visibility(self.window, self.sink_tokens),
+            *self._cache_strides, *self._scale_strides, *self._row_strides, *self._row_strides,
+            _err(step_ctx), step_ctx.stream_handle), "va_window_prefill")
         step_ctx.note_dispatch()
 
     def get_params_dict(self) -> Dict[str, Any]:

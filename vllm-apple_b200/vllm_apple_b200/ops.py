@@ -493,6 +493,13 @@ def _rows(t, name, heads, head_size, rows):
     return st[0], st[1]
 
 
+def visibility(window, sink_tokens) -> tuple[int, int]:
+    """``window`` and ``sink_tokens`` as the library's 32-bit integers: what is past them covers
+    every position there is, and a negative number of sinks stays one (it is refused)."""
+    most = (1 << 31) - 1
+    return min(max(int(window or 0), 0), most), max(min(int(sink_tokens), most), -1)
+
+
 def _new_rows(new_k, new_v, heads, head_size, rows):
     if new_k is None or new_v is None:
         raise ValueError("new_k and new_v go together")
@@ -601,7 +608,7 @@ def paged_window_decode(out, q, k_cache, v_cache, block_table, seq_lens, *, scal
         n_st = _new_rows(new_k, new_v, h, d, B)
     _on(q.device, "out k_cache v_cache block_table seq_lens k_scale v_scale new_k new_v", out,
         k_cache, v_cache, block_table, seq_lens, k_scale, v_scale, new_k, new_v)
-    window = max(int(window or 0), 0)
+    window, sink_tokens = visibility(window, sink_tokens)
     nbytes = _lib.load().va_window_decode_workspace_size(B, Hq, h, d, max_seq_len, window,
                                                          sink_tokens)
     ws = call_workspace(dev, "window_decode", nbytes)
@@ -637,4 +644,4 @@ def paged_window_prefill(out, q, k_cache, v_cache, block_table, query_start_loc,
     _launch(dev, "va_window_prefill", out.data_ptr(), q.data_ptr(), k_cache.data_ptr(),
             v_cache.data_ptr(), _ptr(k_scale), _ptr(v_scale), q8, block_table.data_ptr(),
             query_start_loc.data_ptr(), seq_lens.data_ptr(), T, S, Hq, h, d, bs, mb, nb, scale,
-            max(int(window or 0), 0), sink_tokens, *st, *sc, *q_st, *o_st)
+            *visibility(window, sink_tokens), *st, *sc, *q_st, *o_st)
