@@ -345,12 +345,13 @@ class MetalAttentionImpl(AttentionImpl):
                 ops.kv_write_slots(kc, vc, k3[nd:], v3[nd:], md.slot_mapping[nd:T].contiguous(),
                                    layout="nhd")
             if self._window:
-                # the decode rows are the first nd sequences, one token each
+                # the decode rows are the first nd sequences, one token each; the table may
+                # have more rows than there are sequences
                 ops.paged_window_prefill(o3, q3, kc, vc, bt[nd:],
                                          md.query_start_loc_on(q3.device)[nd:], sl[nd:],
                                          scale=self.scale, window=self._window,
                                          sink_tokens=self.window_sink_tokens, layout="nhd",
-                                         num_seqs=bt.shape[0] - nd)
+                                         num_seqs=sl.numel() - nd)
             else:
                 tok, pos = md.prefill_rows(q3.device)
                 ops.paged_prefill(o3[nd:], q3[nd:], kc, vc, bt, tok, pos, scale=self.scale,
