@@ -432,18 +432,20 @@ def call_workspace(device: int, kind: str, nbytes: int,
 
     Eager calls share :func:`workspace`'s buffer of their stream.  A call that is being
     captured gets its own from the graph's memory pool: two captured graphs may replay
-    at the same time on different streams, so they must not share one."""
+    at the same time on different streams, so they must not share one.  Whether the call
+    is captured is a question to its own stream, which need not be the current one."""
     if not nbytes:
         return None
+    if stream is not None or torch._C._cuda_getDevice() != device:
+        with torch.cuda.stream(torch.cuda.current_stream(device) if stream is None else stream):
+            return call_workspace(device, kind, nbytes)
     if torch._C._cuda_isCurrentStreamCapturing():
-        st = torch.cuda.current_stream(device) if stream is None else stream
-        with torch.cuda.stream(st):
-            return torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
-    if stream is None:  # the usual case, without the lock: the entry is only ever replaced
-        ws = _workspaces.get((device, kind, torch._C._cuda_getCurrentRawStream(device)))
-        if ws is not None and ws.numel() >= nbytes:
-            return ws
-    return workspace(device, kind, nbytes, stream)
+        return torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
+    # the usual case, without the lock: the entry is only ever replaced
+    ws = _workspaces.get((device, kind, torch._C._cuda_getCurrentRawStream(device)))
+    if ws is not None and ws.numel() >= nbytes:
+        return ws
+    return workspace(device, kind, nbytes)
 
 
 def _window_cache(k_cache, v_cache, k_scale, v_scale, layout):
