@@ -21,11 +21,12 @@
 //   * Statistics, sums and O are fp32; P is rounded to fp16 (2^-11 of a value <= 1) for
 //     the second product.  An e4m3 code becomes fp16 exactly; the exponent of a K row
 //     scales its fp32 score, that of a V row its fp16 values (both exact).
-//   * All tiles of the call, in (sequence, head group, tile) order, are one list that is cut
-//     into equal ranges, one per CTA that fits the GPU: ragged lengths, one long sequence or
-//     many short ones all make one even wave.  A range holds whole (sequence, head group)
+//   * Long lists of keys: all tiles of the call, in (sequence, head group, tile) order, are one
+//     list that is cut into equal ranges, one per CTA that fits the GPU, so that ragged lengths
+//     and one long sequence make one even wave.  A range holds whole (sequence, head group)
 //     lists, written at once, and at most two parts of lists, whose (O, m, l) a second
-//     kernel, launched as a programmatic dependent, merges in list order.
+//     kernel, launched as a programmatic dependent, merges in list order.  Short lists and very
+//     many of them have a CTA each instead (make_plan).
 //   * Keys that the query does not see are zero-filled, never read: what lies in the
 //     cache behind a sequence, before its window or in a freed block does not matter.
 // Measured (32 heads of 128 over 8): 128 sequences under a window of 1024, fp16, 95 us (5.6
@@ -709,8 +710,13 @@ constexpr int kMaxPerSm = 4;
 
 // Head groups of up to 16.  All tiles of the call are one list that is cut into equal
 // ranges, one per CTA that fits the GPU at once: one even wave, whatever the lengths.
-// Two cases have nothing to gain from the cut and its merge kernel: sequences of so few
-// tiles that a range is hardly shorter, and so many of them that whole ones balance.
+// Two cases gain nothing from the cut, its search and its merge kernel.  Sequences of at most
+// 40 tiles, which a CTA reads in about that time: 1 to 128 sequences of up to 600 keys, of one
+// length or ragged, take 0.40 to 0.99 of the time cut; of 800 keys 0.72 to 1.18, of 1200 0.84
+// to 1.44.  And so many lists that whole ones balance, ragged ones too, and a CTA that ends
+// makes room for the next one's copies: up to 8192 tokens ragged, fp16 / e4m3 heads of 128,
+// 512 lists 1.20 / 1.34 of the time cut, 1024 1.03 / 1.15, 2048 0.96 / 1.01, 2560 0.95 / 0.99,
+// 4096 0.93 / 0.96, 8192 (1024 sequences of 8 kv heads) 2385 us for 2616 and 1382 for 1506.
 Plan make_plan(int64_t num_seqs, int Hq, int Hkv, int D, int64_t max_len, int window, int sinks) {
   Plan p{};
   const int G = Hq / Hkv;
@@ -723,7 +729,7 @@ Plan make_plan(int64_t num_seqs, int Hq, int Hkv, int D, int64_t max_len, int wi
   // an unaligned run and the sinks each reach into one more tile
   const int64_t tiles = (keys + kKeys - 1) / kKeys + 2;
   const int64_t units = num_seqs * Hkv * p.hg, slots = (int64_t)kMaxPerSm * va_host::sm_count();
-  if (tiles <= 2 * kMinRange || units >= 16 * slots) return p;
+  if (tiles <= 5 * kMinRange || units >= 4 * slots) return p;
   const int64_t most = units * ((tiles + kOpenMost + kMinRange - 1) / kMinRange);
   p.most = (int)(most < slots ? most : slots);
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
