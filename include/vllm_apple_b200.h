@@ -227,7 +227,9 @@ VA_API int va_paged_prefill(void *out, const void *q, const void *k_cache, const
  * A query at position p sees the keys j <= p with p - j < window (window <= 0:
  * every j <= p) or j < sink_tokens.  Blocks that hold no visible key are not
  * read; their block-table entries may hold anything.  Keys that are not visible
- * do not reach the result, whatever their values.
+ * do not reach the result, whatever their values.  Nor does a visible key whose
+ * score is -inf, unless every visible one's is (NaN).  A visible value that is an
+ * infinity or NaN makes its column of the row infinite or NaN.
  * ------------------------------------------------------------------------- */
 
 /* Quantise new K/V rows [num_tokens, num_kv_heads, head_size] (fp16, element

@@ -29,13 +29,17 @@
 //     many of them have a CTA each instead (make_plan).
 //   * Keys that the query does not see are zero-filled, never read: what lies in the
 //     cache behind a sequence, before its window or in a freed block does not matter.
-// Measured (32 heads of 128 over 8): 128 sequences under a window of 1024, fp16, 95 us (5.6
-// TB/s); 128 ragged e4m3 contexts of up to 8192 tokens 211-218 us (5.2 TB/s), one of 131000
-// 60 us (4.5 TB/s).  The copies alone, without products, take 210 and 53 us of the last two,
-// the products alone 132 and 42.  A stream of tiles per warp instead of per CTA took 273 and
-// 74 us, two or eight warps per CTA 269 and 251 us for the contexts, two waves of ranges more
-// than one.  Small calls (4 sequences under a window of 128, 14 heads of 64 over 2: 4.6 us)
-// are launches and one chain of dependent loads.
+// Measured (32 heads of 128 over 8): 128 sequences under a window of 1024, fp16, 94-96 us (5.6
+// TB/s); 128 ragged e4m3 contexts of up to 8192 tokens 207 us (5.4 TB/s; 218-224 called one by
+// one with other inputs each time), one of 131000 59 us (4.6 TB/s).  The copies alone, without
+// products, took 210 and 53 us of the last two when they took 212 and 60, the products alone 132
+// and 42.  A stream of tiles per warp instead of per CTA took 273 and 74 us, two or eight warps
+// per CTA 269 and 251 us for the contexts, two waves of ranges more than one.  Groups of 9 to 16
+// heads (two tiles of columns; 247 to 249 registers at head size 128, so two CTAs per SM where
+// an e4m3 group of up to 8 has three): the same contexts take 361-371 us in fp16 (349 with
+// groups of 4) and 282-294 in e4m3 (207).  Groups of 32 read every key twice: 727 and 577.
+// Small calls (4 sequences under a window of 128, 14 heads of 64 over 2: 4.6 us) are one launch
+// and one chain of dependent loads on a few CTAs.
 #include <float.h>
 
 #include "window.cuh"
@@ -143,9 +147,10 @@ constexpr int kMinRange = 2 * kNW;
 // Beginning another list of tiles (its length, block ids, first copies, the merge of the
 // warps) costs a CTA about as long as 28 tiles, so when the ranges are cut every list
 // counts for that many more: its first `open` places hold no tile.  Three quarters of a range at
-// most, since every range begins one list in any case.  Measured at 4, 16, 28 and 48: 128
-// ragged e4m3 contexts 270 (0), 226, 220, 211 and 222 us; 64 shorter ones, whose ranges are
-// some 30 tiles, 29 us (0), 24 (a quarter of a range), 19.5 (three quarters), 23 (28).
+// most, since every range begins one list in any case.  Measured at 0, 4, 16, 28 and 48: 128
+// ragged e4m3 contexts 270, 226, 220, 211 and 222 us (a build that took 211); 64 shorter ones,
+// whose ranges are some 30 tiles, 29 us (0), 24 (a quarter of a range), 19.5 (three quarters),
+// 23 (28).
 constexpr int kOpenMost = 28;
 VA_DEVINL int places(int tiles, int open) { return tiles > 0 ? tiles + open : 0; }
 
@@ -715,7 +720,7 @@ constexpr int kMaxPerSm = 4;
 // length or ragged, take 0.40 to 0.99 of the time cut; of 800 keys 0.72 to 1.18, of 1200 0.84
 // to 1.44.  And so many lists that whole ones balance, ragged ones too, and a CTA that ends
 // makes room for the next one's copies: up to 8192 tokens ragged, fp16 / e4m3 heads of 128,
-// 512 lists 1.20 / 1.34 of the time cut, 1024 1.03 / 1.15, 2048 0.96 / 1.01, 2560 0.95 / 0.99,
+// 512 lists 1.20 / 1.33 of the time cut, 1024 1.03 / 1.15, 2048 0.96 / 1.01, 2560 0.95 / 0.99,
 // 4096 0.93 / 0.96, 8192 (1024 sequences of 8 kv heads) 2385 us for 2616 and 1382 for 1506.
 Plan make_plan(int64_t num_seqs, int Hq, int Hkv, int D, int64_t max_len, int window, int sinks) {
   Plan p{};

@@ -11,7 +11,9 @@
 //     theirs over with setmaxnreg); P goes back over S as fp16 and feeds the second product
 //     from TMEM.  The maximum a row's powers are taken against only moves when a power
 //     would pass 2^12 (fp16 ends at 2^16), so O is rarely rescaled: 494 us (of 8192 tokens,
-//     below) with 2^6, 480 with 2^8, 476 from 2^10 on.
+//     below) with 2^6, 480 with 2^8, 476 from 2^10 on (before the waits were a warp's).  Rows
+//     whose maximum does move cost what they rescale: 440 us become 488 to 494 with queries 4
+//     to 32 times as large, 65 us (fp16, below) 71 to 72.
 //   * warp 8, one thread: issues tcgen05.mma for both tiles in turn -- PV_0(j-1), S_0(j),
 //     PV_1(j-1), S_1(j) -- so one tile's products run while the other is in its softmax.
 //   * fp16 cache: warp 9 brings K and V key tiles into a ring of shared-memory slots by TMA,
@@ -20,18 +22,20 @@
 //     which gives zeros.  Block sizes that do not tile 128 keys (and cache layouts without a
 //     tensor map) take 16-byte cp.async from warps 12-15 instead, whose issue takes as long as
 //     a tile's products and softmax: four chunks of 512 under a window of 1024 (32 heads of 128
-//     over 8) 67.7 us by TMA, 76.6 by cp.async.
+//     over 8) 65.1 us by TMA, 74.3 by cp.async.
 //   * e4m3 cache: warps 12-19 copy rows by cp.async into a raw buffer two items ahead, and turn
 //     them into fp16 (exactly) in the slot.  TMA into a raw ring was 2 % faster on 8192 tokens
-//     and 2 % slower on short ones; four converting warps took 525 us where eight took 502.
+//     and 2 % slower on short ones; four converting warps took 525 us where eight took 502
+//     (before the waits were a warp's).
 //   Keys that no row of the pair sees are never part of a result: they are zeros, or their
 //   scores are masked for every row.
-// What bounds it: 8192 tokens under a window of 4096 over an e4m3 cache take 476 us (53 % of
-// the measured tensor peak for the visible products).  Alone, on the same grid (of a build
-// that took 491), the products take 368 us, the softmax 376, the conversion 319 and the
-// barriers 223; the products of one tile wait for its softmax, and the overlap of the two
-// tiles hides some of it.  Half-tile double buffering of S, P published in halves and
-// polynomial powers were slower; TMEM is full, so no third tile fits.
+// What bounds it: 8192 tokens under a window of 4096 over an e4m3 cache take 440 us (57 % of
+// the measured tensor peak for the visible products) in a graph's replay, 473 called one by one
+// with other inputs each time; an fp16 cache 398.  Alone, on the same grid, the products take
+// 342 us, the softmax 345, the conversion 369 and the barriers 237; the products of one tile
+// wait for its softmax, and the overlap of the two tiles hides some of it.  Half-tile double
+// buffering of S, P published in halves and polynomial powers were slower; TMEM is full, so no
+// third tile fits.
 // A key masked for one row but seen by another may hold an infinity or a NaN in V, and
 // 0 * inf would reach the masked row.  In key tiles that are masked in part (at most a
 // few per pair) warps 12 on replace such values by 0, and rows that do see them get
@@ -65,8 +69,9 @@ struct Shape {
   static constexpr int kThreads = kFirstProducer + kProducers;
   // Registers: the threads launch with kRegsLaunch each; the warpgroups past the softmax
   // ones go down to kRegsOther and the softmax warpgroups take what they give up.  e4m3, 8192
-  // tokens: 502 us with 168 and 48, 480 with 176 and 40, 510 with 184 and 32; fp16 does not
-  // change from 184 to 208.
+  // tokens (before the waits were a warp's): 502 us with 168 and 48, 480 with 176 and 40, 510
+  // with 184 and 32; fp16 does not change from 184 to 208.  Held to 96 registers at launch, the
+  // e4m3 kernels spill 12 bytes at head size 128 and 8 at 96, the others none.
   static constexpr int kRegsLaunch = Q8 ? 96 : 128, kRegsSoftmax = Q8 ? 176 : 192;
   static constexpr int kRegsOther = Q8 ? 40 : 64;
   static_assert(kThreads * kRegsLaunch <= 65536 &&
@@ -345,9 +350,9 @@ __global__ void __launch_bounds__(Shape<D, Q8, TMA>::kThreads, 1)
   // whether the MMAs that read the item's slot before are done (without waiting; the warp's
   // answer, as above), and a wait
   auto is_empty = [&](int item) {
+    uint64_t *bar = &bar_empty[item % kSlots];
     return item < kSlots ||
-           __all_sync(0xffffffffu,
-                      gone || va::mbar_try_wait(&bar_empty[item % kSlots], ((item / kSlots) - 1) & 1));
+           __all_sync(0xffffffffu, gone || va::mbar_try_wait(bar, ((item / kSlots) - 1) & 1));
   };
   auto wait_empty = [&](int item) {
     if (item >= kSlots) wait_bar(&bar_empty[item % kSlots], ((item / kSlots) - 1) & 1);
