@@ -436,9 +436,14 @@ def call_workspace(device: int, kind: str, nbytes: int,
     is captured is a question to its own stream, which need not be the current one."""
     if not nbytes:
         return None
-    if stream is not None or torch._C._cuda_getDevice() != device:
-        with torch.cuda.stream(torch.cuda.current_stream(device) if stream is None else stream):
-            return call_workspace(device, kind, nbytes)
+    if torch._C._cuda_getDevice() == device and (
+            stream is None or stream.cuda_stream == torch._C._cuda_getCurrentRawStream(device)):
+        return _current_workspace(device, kind, nbytes)
+    with torch.cuda.stream(torch.cuda.current_stream(device) if stream is None else stream):
+        return _current_workspace(device, kind, nbytes)
+
+
+def _current_workspace(device: int, kind: str, nbytes: int) -> torch.Tensor:
     if torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{device}")
     # the usual case, without the lock: the entry is only ever replaced
@@ -499,7 +504,7 @@ def visibility(window, sink_tokens) -> tuple[int, int]:
     """``window`` and ``sink_tokens`` as the library's 32-bit integers: what is past them covers
     every position there is, and a negative number of sinks stays one (it is refused)."""
     most = (1 << 31) - 1
-    return min(max(int(window or 0), 0), most), max(min(int(sink_tokens), most), -1)
+    return min(max(int(window or 0), 0), most), max(min(sink_tokens, most), -1)
 
 
 def _new_rows(new_k, new_v, heads, head_size, rows):
